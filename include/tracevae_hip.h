@@ -43,6 +43,14 @@ extern "C" {
 /* partial operand maxima kept by the caller of tv_gemm_f32_ex */
 #define TV_GEMM_MAX_SLOTS 256
 
+/* element types of the entry points that take more than fp32 */
+#define TV_DTYPE_F32 0
+#define TV_DTYPE_BF16 1
+#define TV_DTYPE_F16 2
+/* tv_adamw_*: elements that share the scale of their 8-bit moments, elements per workgroup */
+#define TV_ADAMW_BLOCK 256
+#define TV_ADAMW_CHUNK 4096
+
 /* status bits written by tv_batch_build into *status (device int32) */
 #define TV_BATCH_TOO_MANY_NODES 1 /* a trace has more than max_node_count nodes           */
 #define TV_BATCH_BAD_EDGE 2       /* an edge violates 0 <= u < v < n                        */
@@ -685,6 +693,59 @@ int tv_optim_step_guarded(int kind, int64_t n, float *param, const float *grad, 
                           int64_t step, const float *guard /* device scalar, nullable */,
                           int guard_kind, float *guard_host /* pinned host scalar, nullable */,
                           void *stream);
+
+/* ------------------------------------------------------------------------------------
+ * AdamW over many tensors where they are (no counterpart in the reference, whose optimizers are
+ * tk.optim RMSprop / Adam, train.py:417-426): decoupled weight decay, clipping by the global norm,
+ * moments in 32 bits or in 8.
+ *   g' = coef g, coef = min(1, clip_norm / (||g|| + 1e-6)) over all tensors (1 if clip_norm = 0;
+ *        a NaN norm gives NaN parameters, as the formula says)
+ *   m = b1 m + (1-b1) g' ; v = b2 v + (1-b2) g'^2
+ *   p = p (1 - lr wd) - lr/(1-b1^t) m / (sqrt(v)/sqrt(1-b2^t) + eps)
+ * Parameters are fp32, bf16 or fp16 (dtypes[i]: TV_DTYPE_*), gradients have the parameter's type.
+ * 16-bit parameters are rounded copies of an fp32 `master` that takes the updates; an element that
+ * is not what its master rounds to was written by somebody else, and the master follows it.
+ *
+ * State: flat buffers of tv_adamw_state_elements() elements in which every tensor begins at a
+ * multiple of TV_ADAMW_BLOCK, in the order of the tensors (elements between two tensors are zero);
+ * caller-owned, 16-byte aligned, zero before the first step:
+ *   state_bits 32: moment1 = m, moment2 = v, fp32; scales NULL
+ *   state_bits  8: moment1 = m / scale1, moment2 = sqrt(v) / scale2, one e4m3 byte each, one fp32
+ *     scale per TV_ADAMW_BLOCK elements = (largest finite magnitude of the block) / 448.  Codes are
+ *     rounded up or down with the probabilities that keep the value on average, by a hash of
+ *     (seed, step, element): same seed, same bits.  A positive sqrt(v) keeps a positive code; an
+ *     infinite or NaN moment becomes the NaN code and leaves its neighbours alone; a block whose
+ *     scale would be below 2^-126 is stored as zeros.
+ *   master: fp32, needed if any parameter has 16 bits (otherwise NULL).
+ *
+ * tv_adamw_plan writes the table of tensors and chunks into HOST memory; the caller keeps it and a
+ *   copy of it in device memory for as long as the parameters stay where they are.  Parameters that
+ *   overlap are refused.
+ * tv_adamw_control writes the image of the control block (tv_adamw_control_bytes) into HOST memory,
+ *   the caller copies it to the device: `step` steps taken, hyper-parameters.  Its layout begins
+ *   with int64 step, double lr, beta1, beta2, eps; a store to lr on the stream sets the rate of the
+ *   steps behind it.  The counter is on the device: a captured step counts on when replayed.
+ * tv_adamw_step: grads is a HOST array of device addresses (NULL: this tensor has no gradient and
+ *   stays as it is, state included), read during the call.  guard / guard_kind / guard_host as in
+ *   tv_optim_step_guarded: a step that is skipped changes nothing, the step counter included.
+ *   norm_out (nullable, device): ||g||, with clip_norm > 0 only.  workspace:
+ *   tv_adamw_workspace_bytes(count) bytes, used with clip_norm > 0 only.  Calls on one state
+ *   must be ordered (one stream, or events).
+ * ---------------------------------------------------------------------------------- */
+int64_t tv_adamw_state_elements(int64_t count, const int64_t *sizes);
+int64_t tv_adamw_plan_bytes(int64_t count, const int64_t *sizes);
+int tv_adamw_plan(int64_t count, const int64_t *sizes, const int *dtypes, void *const *params,
+                  const double *weight_decay, void *plan, int64_t plan_bytes);
+int64_t tv_adamw_control_bytes(void);
+int tv_adamw_control(int64_t step, double lr, double beta1, double beta2, double eps, void *control);
+int64_t tv_adamw_workspace_bytes(int64_t count);
+int tv_adamw_step(const void *plan_host, const void *plan_device, const void *const *grads,
+                  int state_bits, void *moment1, void *moment2, float *scale1 /* nullable */,
+                  float *scale2 /* nullable */, float *master /* nullable */, void *control,
+                  double clip_norm, double *norm_out /* nullable */, int64_t seed,
+                  const float *guard /* nullable */, int guard_kind,
+                  float *guard_host /* pinned host scalar, nullable */, void *workspace,
+                  int64_t workspace_bytes, void *stream);
 
 /* ------------------------------------------------------------------------------------
  * the scalar end of train_step (tracegnn/models/trace_vae/train.py:229-270):

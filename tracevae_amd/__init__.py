@@ -15,7 +15,7 @@ __all__ = [
     'constants', 'ExpConfig', 'TraceVAEConfig', 'TraceStructVAEConfig', 'TraceLatencyVAEConfig',
     'parse_flags', 'FlatTraces', 'TraceGraph', 'TraceGraphNode', 'TraceGraphNodeFeatures',
     'TraceGraphIDManager', 'TraceGraphLatencyRangeFile', 'flatten_trace_graphs',
-    'TraceGraphBatch', 'DeviceTraceStore', 'TraceVAE',
+    'TraceGraphBatch', 'DeviceTraceStore', 'TraceVAE', 'AdamW',
 ]
 
 
@@ -27,4 +27,7 @@ def __getattr__(name):
     if name == 'TraceVAE':
         from .model import TraceVAE
         return TraceVAE
+    if name == 'AdamW':
+        from .optim import AdamW
+        return AdamW
     raise AttributeError(name)

@@ -187,7 +187,8 @@ class ExpConfig(Config):
         init_batch_size = 64
         batch_size = 64
         val_batch_size = 64
-        optimizer = 'rmsprop'    # 'adam' | 'rmsprop'
+        optimizer = 'rmsprop'    # 'adam' | 'rmsprop'; not in the reference: 'adamw' | 'adamw8'
+        weight_decay = 0.01      # of 'adamw' / 'adamw8' (biases are left out)
         initial_lr = 0.001
         lr_anneal_ratio = 0.1
         lr_anneal_epochs = 30

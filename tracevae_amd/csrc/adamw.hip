@@ -1,0 +1,567 @@
+// AdamW over many tensors at once: global gradient norm, clipping, decoupled weight decay and the
+// moments in 32 bits or in 8 bits with one fp32 scale per block of 256 elements.
+//
+//   g' = coef g,  coef = min(1, clip / (||g|| + 1e-6))
+//   m  = b1 m + (1 - b1) g',  v = b2 v + (1 - b2) g'^2
+//   p  = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// The tensors stay where they are: a plan in device memory lists them and cuts each one into chunks
+// of 4096 elements, one workgroup per chunk; the gradients' addresses, which autograd changes from
+// step to step, travel as kernel arguments.  Everything is elementwise and bound by HBM: 28 bytes
+// per fp32 parameter with 32-bit moments, 16.06 with 8-bit ones.
+//
+// 8-bit moments: m / s_m and sqrt(v) / s_r in e4m3 with s = max over the block / 448, so that the
+// largest element sits on the largest code.  The codes are rounded STOCHASTICALLY, from a hash of
+// (seed, step, element): one step moves v by (1 - b2) = 0.1 % of itself, half the distance of two
+// codes is up to 6 %, so rounding to nearest would never move most elements again.  The arithmetic
+// up to the code is in float64, so that which of two neighbouring codes is taken does not hang on the
+// rounding of an intermediate; the moments that move the parameter are the ones before rounding.
+#include <math.h>
+
+#include <algorithm>
+#include <memory>
+#include <new>
+
+#include "tv_common.h"
+
+namespace {
+
+constexpr int AW_THREADS = 256;
+constexpr int AW_CHUNK = TV_ADAMW_CHUNK;          // elements per workgroup
+constexpr int AW_BLOCK = TV_ADAMW_BLOCK;          // elements per scale: one wave, 4 per lane
+constexpr int AW_GRADS = 384;                     // gradient addresses per launch (3 KB of arguments)
+constexpr int AW_NORM_BLOCKS = 2048;              // partial sums per launch
+constexpr int64_t AW_MAGIC = 0x74765f6164616d77;
+
+struct Tensor {
+  void *param;
+  int64_t n;
+  int64_t state;                                  // first element of its segment of the state
+  double weight_decay;
+  int32_t dtype;
+  int32_t first_chunk;
+};
+struct Chunk {
+  int32_t tensor, index;
+};
+struct Plan {                                     // tensors and chunks follow
+  int64_t magic, count, chunks, elements;
+};
+struct Control {
+  int64_t step;                                   // steps taken
+  double lr, beta1, beta2, eps;
+  double beta1_t, beta2_t;                        // beta^step
+  // of the step being taken, written by begin_kernel
+  double norm, coef;
+  float step_size, inv_sqrt_bc2, eps_f;
+  int32_t skip;
+};
+struct Grads {
+  const void *g[AW_GRADS];
+};
+
+__host__ __device__ inline const Tensor *plan_tensors(const void *plan) {
+  return reinterpret_cast<const Tensor *>(static_cast<const char *>(plan) + sizeof(Plan));
+}
+__host__ __device__ inline const Chunk *plan_chunks(const void *plan, int64_t count) {
+  return reinterpret_cast<const Chunk *>(static_cast<const char *>(plan) + sizeof(Plan) +
+                                         count * (int64_t)sizeof(Tensor));
+}
+
+// four consecutive elements from i on, zeros behind n
+template <typename T>
+__device__ __forceinline__ void load4(const T *p, int i, int n, bool aligned, float (&x)[4]) {
+  if (aligned && i + 4 <= n) {
+    typedef T Vec __attribute__((ext_vector_type(4)));
+    const Vec f = *reinterpret_cast<const Vec *>(p + i);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = (float)f[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = i + j < n ? (float)p[i + j] : 0.f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store4(T *p, int i, int n, bool aligned, const float (&x)[4]) {
+  if (aligned && i + 4 <= n) {
+    typedef T Vec __attribute__((ext_vector_type(4)));
+    Vec f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = (T)x[j];
+    *reinterpret_cast<Vec *>(p + i) = f;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i + j < n) p[i + j] = (T)x[j];
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// ||g||: float64 squares, one partial per workgroup, summed in order by begin_kernel
+// ---------------------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ double chunk_sumsq(const T *g, int n) {
+  const bool aligned = (((uintptr_t)g) & (4 * sizeof(T) - 1)) == 0;
+  double acc = 0.0;
+#pragma unroll
+  for (int it = 0; it < AW_CHUNK / (4 * AW_THREADS); ++it) {
+    const int i = it * 4 * AW_THREADS + (int)threadIdx.x * 4;
+    if (i < n) {
+      float x[4];
+      load4(g, i, n, aligned, x);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc = fma((double)x[j], (double)x[j], acc);
+    }
+  }
+  return acc;
+}
+
+__global__ __launch_bounds__(AW_THREADS) void adamw_sumsq_kernel(const void *plan, int64_t count,
+                                                                 int64_t chunk0, int64_t chunk1,
+                                                                 int64_t tensor0, Grads grads,
+                                                                 double *__restrict__ partial) {
+  __shared__ double red[AW_THREADS / 64];
+  const Tensor *tensors = plan_tensors(plan);
+  const Chunk *chunks = plan_chunks(plan, count);
+  double acc = 0.0;
+  for (int64_t c = chunk0 + blockIdx.x; c < chunk1; c += gridDim.x) {
+    const Chunk ch = chunks[c];
+    const Tensor t = tensors[ch.tensor];
+    const int64_t base = (int64_t)ch.index * AW_CHUNK;
+    const int n = (int)(t.n - base < AW_CHUNK ? t.n - base : AW_CHUNK);
+    const void *g = grads.g[ch.tensor - tensor0];
+    if (g == nullptr) continue;
+    if (t.dtype == TV_DTYPE_F32) acc += chunk_sumsq((const float *)g + base, n);
+    else if (t.dtype == TV_DTYPE_BF16) acc += chunk_sumsq((const __bf16 *)g + base, n);
+    else acc += chunk_sumsq((const _Float16 *)g + base, n);
+  }
+  acc = tv_wave_sum_d(acc);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = acc;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double s = red[0];
+    for (int w = 1; w < AW_THREADS / 64; ++w) s += red[w];
+    partial[blockIdx.x] = s;
+  }
+}
+
+// The scalars of one step: norm and clip coefficient, the NaN decision, bias corrections.  The step
+// counter and the learning rate live on the device, so a captured step counts on when it is replayed.
+__global__ __launch_bounds__(256) void adamw_begin_kernel(Control *ctl, bool clipped, int64_t nblk,
+                                                          const double *__restrict__ partial,
+                                                          double clip, double *norm_out,
+                                                          const float *guard, int guard_kind,
+                                                          float *guard_copy) {
+  __shared__ double red[256];
+  double acc = 0.0;
+  for (int64_t i = threadIdx.x; i < nblk; i += 256) acc += partial[i];
+  red[threadIdx.x] = acc;
+  __syncthreads();
+  for (int s = 128; s > 0; s >>= 1) {
+    if ((int)threadIdx.x < s) red[threadIdx.x] += red[threadIdx.x + s];
+    __syncthreads();
+  }
+  if (threadIdx.x != 0) return;
+  double coef = 1.0;
+  if (clipped) {
+    const double norm = sqrt(red[0]);
+    ctl->norm = norm;
+    if (norm_out != nullptr) norm_out[0] = norm;
+    // a NaN norm gives a NaN coefficient, and so NaN parameters
+    coef = clip / (norm + 1e-6);
+    if (coef > 1.0) coef = 1.0;
+  }
+  ctl->coef = coef;
+  bool skip = false;
+  if (guard != nullptr) {
+    const float v = guard[0];
+    if (guard_copy != nullptr) guard_copy[0] = v;
+    skip = guard_kind == 1 ? (v != v) : (v != 0.f);
+  }
+  ctl->skip = skip ? 1 : 0;
+  if (skip) return;
+  const double b1t = ctl->beta1_t * ctl->beta1, b2t = ctl->beta2_t * ctl->beta2;
+  ctl->step += 1;
+  ctl->beta1_t = b1t;
+  ctl->beta2_t = b2t;
+  ctl->step_size = (float)(ctl->lr / (1.0 - b1t));
+  ctl->inv_sqrt_bc2 = (float)(1.0 / sqrt(1.0 - b2t));
+  ctl->eps_f = (float)ctl->eps;
+}
+
+// ---------------------------------------------------------------------------------------
+// the update
+// ---------------------------------------------------------------------------------------
+struct Step {
+  float keep, step_size, inv_sqrt_bc2, eps;       // keep = 1 - lr * weight_decay
+  double coef, beta1, beta2, omb1, omb2;
+  uint32_t key;
+};
+
+__device__ __forceinline__ float moved(float p, float m, float r, const Step &s) {
+  float x = fmaf(-s.step_size, m / fmaf(r, s.inv_sqrt_bc2, s.eps), p * s.keep);
+  // the fp32 value itself: the compiler would fold a conversion to fp16 into the fma, and the
+  // parameter would no longer be what its master rounds to
+  asm("" : "+v"(x));
+  return x;
+}
+
+// 16-bit parameters are rounded copies of an fp32 master; one that is not what its master rounds to
+// was written by somebody else (a checkpoint was loaded), and the master follows it
+template <typename T>
+__device__ __forceinline__ float master_of(float p, float w) {
+  return (float)(T)w == p ? w : p;
+}
+template <>
+__device__ __forceinline__ float master_of<float>(float p, float) { return p; }
+
+template <typename T>
+__device__ __forceinline__ void chunk_step32(T *p, const T *g, float *w, float *m, float *v, int n,
+                                             const Step &s) {
+  const bool aligned = ((((uintptr_t)g) | (uintptr_t)p) & (4 * sizeof(T) - 1)) == 0;
+  const float b1 = (float)s.beta1, b2 = (float)s.beta2, o1 = (float)s.omb1, o2 = (float)s.omb2;
+  const float coef = (float)s.coef;
+  for (int it = 0; it < AW_CHUNK / (4 * AW_THREADS); ++it) {
+    const int i = it * 4 * AW_THREADS + (int)threadIdx.x * 4;
+    if (i >= n) continue;
+    float px[4], gx[4], wx[4], mx[4], vx[4];
+    load4(p, i, n, aligned, px);
+    load4(g, i, n, aligned, gx);
+    load4(m, i, AW_CHUNK, true, mx);              // (segments of the state are padded to 256)
+    load4(v, i, AW_CHUNK, true, vx);
+    if (sizeof(T) != 4) load4(w, i, AW_CHUNK, true, wx);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float gj = gx[j] * coef;
+      mx[j] = fmaf(b1, mx[j], o1 * gj);
+      vx[j] = fmaf(b2, vx[j], o2 * gj * gj);
+      px[j] = moved(sizeof(T) == 4 ? px[j] : master_of<T>(px[j], wx[j]), mx[j], sqrtf(vx[j]), s);
+    }
+    store4(p, i, n, aligned, px);
+    store4(m, i, AW_CHUNK, true, mx);
+    store4(v, i, AW_CHUNK, true, vx);
+    if (sizeof(T) != 4) store4(w, i, AW_CHUNK, true, px);
+  }
+}
+
+__host__ __device__ inline uint32_t mix(uint32_t x) {
+  // two rounds of shift and multiply by odd constants (fractional bits of sqrt 2 and sqrt 3)
+  x ^= x >> 16;
+  x *= 0x6a09e667u;
+  x ^= x >> 15;
+  x *= 0xbb67ae85u;
+  return x ^ (x >> 16);
+}
+
+// e4m3 magnitude code of y in [0, 448 (1 + 2^-23)], rounded up with the probability of what is left
+// over the code below: 17 random bits (the lowest always set, so an exact value stays) are added to
+// the 17 mantissa bits of the high word that e4m3 drops.  Below 2^-6 codes lie 2^-9 apart: adding
+// 2^-6 puts those bits at the same place.
+__device__ __forceinline__ uint32_t code_of(double y, uint32_t random16) {
+  const bool low = y < 0.015625;
+  const double z = low ? y + 0.015625 : y;
+  const uint32_t hi = (uint32_t)__double2hiint(z) + (2 * random16 + 1);
+  const uint32_t c = (hi >> 17) - (1016u << 3) - (low ? 8u : 0u);
+  return c < 126u ? c : 126u;
+}
+__device__ __forceinline__ float scale_of(float largest) {
+  const float s = largest / 448.f;
+  return s >= 1.17549435e-38f ? s : 0.f;          // (below that the block counts as zero)
+}
+__device__ __forceinline__ bool finite(double x) {
+  return (__double2hiint(x) & 0x7ff00000) != 0x7ff00000;
+}
+__device__ __forceinline__ void decode4(uint32_t c, float (&x)[4]) {
+  typedef float F2 __attribute__((ext_vector_type(2)));
+  const F2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false);
+  const F2 b = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);
+  x[0] = a[0]; x[1] = a[1]; x[2] = b[0]; x[3] = b[1];
+}
+
+template <typename T>
+__device__ __forceinline__ void chunk_step8(T *p, const T *g, float *w, uint32_t *m8, float *ms,
+                                            uint32_t *r8, float *rs, int n, int64_t element0,
+                                            const Step &s) {
+  const bool aligned = ((((uintptr_t)g) | (uintptr_t)p) & (4 * sizeof(T) - 1)) == 0;
+  const int lane = threadIdx.x & 63;
+  for (int it = 0; it < AW_CHUNK / (4 * AW_THREADS); ++it) {
+    const int i = it * 4 * AW_THREADS + (int)threadIdx.x * 4;
+    const int b = i / AW_BLOCK;
+    if (b * AW_BLOCK >= n) continue;              // (the same for the whole wave)
+    // (blocks begin at multiples of 256: the high word is the same for the whole block)
+    const uint32_t key = mix(s.key + (uint32_t)((element0 + b * AW_BLOCK) >> 32));
+    const uint32_t element = (uint32_t)(element0 + i);
+    float px[4], gx[4], wx[4], mo[4], ro[4];
+    load4(p, i, n, aligned, px);
+    load4(g, i, n, aligned, gx);
+    decode4(m8[i / 4], mo);
+    decode4(r8[i / 4], ro);
+    if (sizeof(T) != 4) load4(w, i, AW_CHUNK, true, wx);
+    const double sm = ms[b], sr = rs[b];
+    double mx[4], rx[4];
+    float am = 0.f, ar = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const double gj = (double)gx[j] * s.coef;
+      const double ro_ = ro[j] * sr;
+      mx[j] = fma(s.beta1, mo[j] * sm, s.omb1 * gj);
+      rx[j] = sqrt(fma(s.beta2, ro_ * ro_, s.omb2 * gj * gj));
+      if (finite(mx[j])) am = fmaxf(am, (float)fabs(mx[j]));
+      if (finite(rx[j])) ar = fmaxf(ar, (float)rx[j]);
+    }
+    am = tv_wave_max(am);
+    ar = tv_wave_max(ar);
+    const float nm = scale_of(am), nr = scale_of(ar);
+    const double im = nm > 0.f ? 1.0 / (double)nm : 0.0, ir = nr > 0.f ? 1.0 / (double)nr : 0.0;
+    uint32_t cm = 0, cr = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t u = mix(key ^ (element + (uint32_t)j));
+      uint32_t a = 127u, c = 127u;                // NaN
+      if (finite(mx[j])) a = code_of(fabs(mx[j]) * im, u & 0xffffu);
+      if (finite(rx[j])) {
+        c = code_of(rx[j] * ir, u >> 16);
+        if (c == 0u && rx[j] > 0.0) c = 1u;       // a positive rms stays positive
+      }
+      a |= ((uint32_t)__double2hiint(mx[j]) >> 24) & 0x80u;
+      cm |= a << (8 * j);
+      cr |= c << (8 * j);
+      px[j] = moved(sizeof(T) == 4 ? px[j] : master_of<T>(px[j], wx[j]), (float)mx[j], (float)rx[j], s);
+    }
+    store4(p, i, n, aligned, px);
+    if (sizeof(T) != 4) store4(w, i, AW_CHUNK, true, px);
+    m8[i / 4] = cm;
+    r8[i / 4] = cr;
+    if (lane == 0) {
+      ms[b] = nm;
+      rs[b] = nr;
+    }
+  }
+}
+
+template <bool EIGHT>
+__global__ __launch_bounds__(AW_THREADS) void adamw_step_kernel(
+    const void *plan, int64_t count, int64_t chunk0, int64_t tensor0, Grads grads,
+    const Control *__restrict__ ctl, void *moment1, void *moment2, float *scale1, float *scale2,
+    float *master, uint32_t seed_key) {
+  if (ctl->skip) return;
+  const Chunk ch = plan_chunks(plan, count)[chunk0 + blockIdx.x];
+  const Tensor t = plan_tensors(plan)[ch.tensor];
+  const void *g = grads.g[ch.tensor - tensor0];
+  if (g == nullptr) return;                       // no gradient: the tensor stays as it is
+  const int64_t base = (int64_t)ch.index * AW_CHUNK, at = t.state + base;
+  const int n = (int)(t.n - base < AW_CHUNK ? t.n - base : AW_CHUNK);
+  Step s;
+  s.keep = (float)(1.0 - ctl->lr * t.weight_decay);
+  s.step_size = ctl->step_size;
+  s.inv_sqrt_bc2 = ctl->inv_sqrt_bc2;
+  s.eps = ctl->eps_f;
+  s.coef = ctl->coef;
+  s.beta1 = ctl->beta1;
+  s.beta2 = ctl->beta2;
+  s.omb1 = 1.0 - s.beta1;
+  s.omb2 = 1.0 - s.beta2;
+  float *w = master ? master + at : nullptr;
+  if (EIGHT) {
+    s.key = mix(seed_key + (uint32_t)ctl->step);
+    uint32_t *m8 = (uint32_t *)moment1 + at / 4, *r8 = (uint32_t *)moment2 + at / 4;
+    float *ms = scale1 + at / AW_BLOCK, *rs = scale2 + at / AW_BLOCK;
+    if (t.dtype == TV_DTYPE_F32)
+      chunk_step8((float *)t.param + base, (const float *)g + base, w, m8, ms, r8, rs, n, at, s);
+    else if (t.dtype == TV_DTYPE_BF16)
+      chunk_step8((__bf16 *)t.param + base, (const __bf16 *)g + base, w, m8, ms, r8, rs, n, at, s);
+    else
+      chunk_step8((_Float16 *)t.param + base, (const _Float16 *)g + base, w, m8, ms, r8, rs, n, at, s);
+  } else {
+    float *m = (float *)moment1 + at, *v = (float *)moment2 + at;
+    if (t.dtype == TV_DTYPE_F32)
+      chunk_step32((float *)t.param + base, (const float *)g + base, w, m, v, n, s);
+    else if (t.dtype == TV_DTYPE_BF16)
+      chunk_step32((__bf16 *)t.param + base, (const __bf16 *)g + base, w, m, v, n, s);
+    else
+      chunk_step32((_Float16 *)t.param + base, (const _Float16 *)g + base, w, m, v, n, s);
+  }
+}
+
+inline int64_t padded(int64_t n) { return tv_cdiv(n, AW_BLOCK) * AW_BLOCK; }
+inline int64_t groups(int64_t count) { return tv_cdiv(count, AW_GRADS); }
+
+}  // namespace
+
+extern "C" int64_t tv_adamw_control_bytes(void) { return (int64_t)sizeof(Control); }
+
+extern "C" int tv_adamw_control(int64_t step, double lr, double beta1, double beta2, double eps,
+                                void *control) {
+  TV_REQUIRE(control, "tv_adamw_control: null pointer");
+  TV_REQUIRE(step >= 0, "tv_adamw_control: step counts from 0 (steps taken so far)");
+  TV_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0,
+             "tv_adamw_control: the betas lie in [0, 1)");
+  TV_REQUIRE(eps >= 0.0 && lr >= 0.0, "tv_adamw_control: lr and eps are not negative");
+  Control c = {};
+  c.step = step;
+  c.lr = lr;
+  c.beta1 = beta1;
+  c.beta2 = beta2;
+  c.eps = eps;
+  c.beta1_t = pow(beta1, (double)step);
+  c.beta2_t = pow(beta2, (double)step);
+  *(Control *)control = c;
+  return TV_OK;
+}
+
+extern "C" int64_t tv_adamw_state_elements(int64_t count, const int64_t *sizes) {
+  if (count < 1 || !sizes) return -1;
+  int64_t total = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    if (sizes[i] < 0 || sizes[i] > INT64_MAX / 16 - total) return -1;
+    total += padded(sizes[i]);
+  }
+  return total;
+}
+
+extern "C" int64_t tv_adamw_plan_bytes(int64_t count, const int64_t *sizes) {
+  if (tv_adamw_state_elements(count, sizes) < 0) return -1;
+  int64_t chunks = 0;
+  for (int64_t i = 0; i < count; ++i) chunks += tv_cdiv(sizes[i], AW_CHUNK);
+  return (int64_t)sizeof(Plan) + count * (int64_t)sizeof(Tensor) + chunks * (int64_t)sizeof(Chunk);
+}
+
+extern "C" int tv_adamw_plan(int64_t count, const int64_t *sizes, const int *dtypes,
+                             void *const *params, const double *weight_decay, void *plan,
+                             int64_t plan_bytes) {
+  TV_REQUIRE(count >= 1 && sizes && dtypes && params && weight_decay && plan,
+             "tv_adamw_plan: bad arguments");
+  const int64_t need = tv_adamw_plan_bytes(count, sizes);
+  TV_REQUIRE(need >= 0, "tv_adamw_plan: a size is negative or the sizes are too large");
+  TV_REQUIRE((need - (int64_t)sizeof(Plan) - count * (int64_t)sizeof(Tensor)) / (int64_t)sizeof(Chunk) <= INT32_MAX,
+             "tv_adamw_plan: more than 2^31 chunks of %d elements", AW_CHUNK);
+  if (plan_bytes < need) {
+    tv_set_error("tv_adamw_plan: plan of %lld bytes, %lld needed", (long long)plan_bytes, (long long)need);
+    return TV_ERR_WORKSPACE;
+  }
+  Tensor *tensors = const_cast<Tensor *>(plan_tensors(plan));
+  Chunk *chunks = const_cast<Chunk *>(plan_chunks(plan, count));
+  int64_t chunk = 0, state = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    const int width = dtypes[i] == TV_DTYPE_F32 ? 4 : 2;
+    TV_REQUIRE(dtypes[i] == TV_DTYPE_F32 || dtypes[i] == TV_DTYPE_BF16 || dtypes[i] == TV_DTYPE_F16,
+               "tv_adamw_plan: tensor %lld has an unknown dtype %d", (long long)i, dtypes[i]);
+    TV_REQUIRE((params[i] || sizes[i] == 0) && ((uintptr_t)params[i] & (uintptr_t)(width - 1)) == 0,
+               "tv_adamw_plan: tensor %lld has a null or misaligned address", (long long)i);
+    TV_REQUIRE(weight_decay[i] >= 0.0, "tv_adamw_plan: the weight decay of tensor %lld is negative",
+               (long long)i);
+    Tensor t = {};
+    t.param = params[i];
+    t.n = sizes[i];
+    t.state = state;
+    t.weight_decay = weight_decay[i];
+    t.dtype = dtypes[i];
+    t.first_chunk = (int32_t)chunk;
+    tensors[i] = t;
+    for (int64_t k = 0; k < tv_cdiv(sizes[i], AW_CHUNK); ++k) {
+      TV_REQUIRE(k <= INT32_MAX, "tv_adamw_plan: a tensor has too many chunks");
+      chunks[chunk++] = Chunk{(int32_t)i, (int32_t)k};
+    }
+    state += padded(sizes[i]);
+  }
+  // two tensors in one place would be updated twice, at once
+  struct Span {
+    uintptr_t first, last;
+    bool operator<(const Span &o) const { return first < o.first; }
+  };
+  std::unique_ptr<Span[]> spans(new (std::nothrow) Span[(size_t)count]);
+  TV_REQUIRE(spans, "tv_adamw_plan: out of host memory");
+  int64_t used = 0;
+  for (int64_t i = 0; i < count; ++i)
+    if (sizes[i] > 0)
+      spans[used++] = {(uintptr_t)params[i],
+                       (uintptr_t)params[i] + (uintptr_t)sizes[i] * (dtypes[i] == TV_DTYPE_F32 ? 4 : 2)};
+  std::sort(spans.get(), spans.get() + used);
+  for (int64_t i = 1; i < used; ++i)
+    TV_REQUIRE(spans[i].first >= spans[i - 1].last, "tv_adamw_plan: two tensors overlap in memory");
+  Plan head = {AW_MAGIC, count, chunk, state};
+  *(Plan *)plan = head;
+  return TV_OK;
+}
+
+extern "C" int64_t tv_adamw_workspace_bytes(int64_t count) {
+  return groups(count < 1 ? 1 : count) * AW_NORM_BLOCKS * (int64_t)sizeof(double);
+}
+
+extern "C" int tv_adamw_step(const void *plan_host, const void *plan_device,
+                             const void *const *grads, int state_bits, void *moment1, void *moment2,
+                             float *scale1, float *scale2, float *master, void *control,
+                             double clip_norm, double *norm_out, int64_t seed, const float *guard,
+                             int guard_kind, float *guard_host, void *workspace,
+                             int64_t workspace_bytes, void *stream) {
+  TV_REQUIRE(plan_host && plan_device && grads && control, "tv_adamw_step: null pointer");
+  const Plan *plan = (const Plan *)plan_host;
+  TV_REQUIRE(plan->magic == AW_MAGIC, "tv_adamw_step: not a plan of tv_adamw_plan");
+  TV_REQUIRE(state_bits == 8 || state_bits == 32, "tv_adamw_step: moments of 8 or 32 bits");
+  TV_REQUIRE((moment1 && moment2) || plan->elements == 0, "tv_adamw_step: null moments");
+  TV_REQUIRE(state_bits == 32 || (scale1 && scale2) || plan->elements == 0,
+             "tv_adamw_step: 8-bit moments need their scales");
+  TV_REQUIRE(((((uintptr_t)moment1) | (uintptr_t)moment2 | (uintptr_t)master) & 15) == 0,
+             "tv_adamw_step: moments and master are 16-byte aligned");
+  TV_REQUIRE(clip_norm >= 0.0, "tv_adamw_step: clip_norm is 0 (off) or positive");
+  TV_REQUIRE(clip_norm > 0.0 || !norm_out, "tv_adamw_step: the norm is computed with clip_norm only");
+  TV_REQUIRE(guard_kind >= 0 && guard_kind <= 2 && (guard != nullptr) == (guard_kind != 0),
+             "tv_adamw_step: guard_kind 1 (NaN) or 2 (non-zero) with a guard, 0 without");
+  TV_REQUIRE(!guard_host || guard, "tv_adamw_step: guard_host without a guard");
+  const Tensor *tensors = plan_tensors(plan_host);
+  for (int64_t i = 0; i < plan->count; ++i) {
+    TV_REQUIRE(((uintptr_t)grads[i] & (tensors[i].dtype == TV_DTYPE_F32 ? 3 : 1)) == 0,
+               "tv_adamw_step: the gradient of tensor %lld is misaligned", (long long)i);
+    TV_REQUIRE(tensors[i].dtype == TV_DTYPE_F32 || master || tensors[i].n == 0,
+               "tv_adamw_step: 16-bit parameters need a master");
+  }
+  const int64_t ngroups = groups(plan->count);
+  if (clip_norm > 0.0) {
+    TV_REQUIRE(workspace, "tv_adamw_step: null workspace");
+    if (workspace_bytes < tv_adamw_workspace_bytes(plan->count)) {
+      tv_set_error("tv_adamw_step: workspace too small");
+      return TV_ERR_WORKSPACE;
+    }
+  }
+  float *guard_copy = nullptr;
+  if (guard_host) {
+    const int rc = tv_pinned_pointer("tv_adamw_step", guard_host, &guard_copy);
+    if (rc != TV_OK) return rc;
+  }
+  auto group_grads = [&](int64_t k, Grads &g, int64_t &chunk0, int64_t &chunk1) {
+    const int64_t t0 = k * AW_GRADS, t1 = t0 + AW_GRADS < plan->count ? t0 + AW_GRADS : plan->count;
+    for (int64_t i = t0; i < t1; ++i) g.g[i - t0] = grads[i];
+    chunk0 = tensors[t0].first_chunk;
+    chunk1 = t1 < plan->count ? tensors[t1].first_chunk : plan->chunks;
+  };
+  int64_t nblk = 0;
+  double *partial = (double *)workspace;
+  for (int64_t k = 0; clip_norm > 0.0 && k < ngroups; ++k) {
+    Grads g = {};
+    int64_t c0, c1;
+    group_grads(k, g, c0, c1);
+    if (c1 == c0) continue;
+    const int64_t blocks = c1 - c0 < AW_NORM_BLOCKS ? c1 - c0 : AW_NORM_BLOCKS;
+    hipLaunchKernelGGL(adamw_sumsq_kernel, dim3((unsigned)blocks), dim3(AW_THREADS), 0,
+                       (hipStream_t)stream, plan_device, plan->count, c0, c1, k * AW_GRADS, g,
+                       partial + nblk);
+    TV_LAUNCH_CHECK("tv_adamw_step");
+    nblk += blocks;
+  }
+  hipLaunchKernelGGL(adamw_begin_kernel, dim3(1), dim3(256), 0, (hipStream_t)stream,
+                     (Control *)control, clip_norm > 0.0, nblk, partial, clip_norm, norm_out, guard,
+                     guard_kind, guard_copy);
+  TV_LAUNCH_CHECK("tv_adamw_step");
+  for (int64_t k = 0; k < ngroups; ++k) {
+    Grads g = {};
+    int64_t c0, c1;
+    group_grads(k, g, c0, c1);
+    if (c1 == c0) continue;
+    auto kernel = state_bits == 8 ? adamw_step_kernel<true> : adamw_step_kernel<false>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(c1 - c0)), dim3(AW_THREADS), 0, (hipStream_t)stream,
+                       plan_device, plan->count, c0, k * AW_GRADS, g, (const Control *)control,
+                       moment1, moment2, scale1, scale2, master, mix((uint32_t)seed));
+    TV_LAUNCH_CHECK("tv_adamw_step");
+  }
+  return TV_OK;
+}

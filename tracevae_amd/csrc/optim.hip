@@ -196,6 +196,18 @@ extern "C" int tv_axpy_masked(int64_t n, float alpha, const float *x, const uint
   return TV_OK;
 }
 
+int tv_pinned_pointer(const char *who, float *host, float **mapped) {
+  void *p = nullptr;
+  const hipError_t e = hipHostGetDevicePointer(&p, host, 0);
+  if (e != hipSuccess || !p) {
+    (void)hipGetLastError();   // the refusal is ours to report: leave no sticky HIP error behind
+    tv_set_error("%s: guard_host is not pinned host memory (%s)", who, hipGetErrorString(e));
+    return TV_ERR_INVALID;
+  }
+  *mapped = (float *)p;
+  return TV_OK;
+}
+
 static int optim_step(const char *who, int kind, int64_t n, float *param, const float *grad,
                       float *state1, float *state2, const float *grad_norm, float clip_norm,
                       float lr, float beta1, float beta2, float eps, int64_t step,
@@ -209,17 +221,8 @@ static int optim_step(const char *who, int kind, int64_t n, float *param, const 
   TV_REQUIRE(!guard_host || guard, "tv_optim_step_guarded: guard_host without a guard");
   float *guard_copy = nullptr;
   if (guard_host) {
-    // the device's address of the pinned host scalar; fails (instead of faulting in the kernel)
-    // for memory that is not mapped
-    void *mapped = nullptr;
-    const hipError_t e = hipHostGetDevicePointer(&mapped, guard_host, 0);
-    if (e != hipSuccess || !mapped) {
-      (void)hipGetLastError();   // the refusal is ours to report: leave no sticky HIP error behind
-      tv_set_error("tv_optim_step_guarded: guard_host is not pinned host memory (%s)",
-                   hipGetErrorString(e));
-      return TV_ERR_INVALID;
-    }
-    guard_copy = (float *)mapped;
+    const int rc = tv_pinned_pointer("tv_optim_step_guarded", guard_host, &guard_copy);
+    if (rc != TV_OK) return rc;
   }
   float bc1 = 1.0f, bc2s = 1.0f;
   if (kind == 1) {

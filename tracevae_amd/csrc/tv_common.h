@@ -11,6 +11,9 @@
 #define TV_WAVE 64
 
 void tv_set_error(const char *fmt, ...);
+// the device's address of a pinned host scalar; TV_ERR_INVALID (with the error text set) for host
+// memory that is not mapped, where a kernel's store would fault
+int tv_pinned_pointer(const char *who, float *host, float **mapped);
 
 #define TV_REQUIRE(cond, ...)            \
   do {                                   \

@@ -33,7 +33,7 @@ def header_path() -> str:
 def _parse_header(path: str) -> Dict[str, str]:
     """Derive the ctypes signatures from the C declarations, so that the binding cannot
     drift from `include/tracevae_hip.h`.
-    i = int, l = int64, f = float, p = pointer, s = stream (last `void *stream`), c = char*."""
+    i = int, l = int64, f = float, d = double, p = pointer, s = stream (last `void *stream`), c = char*."""
     import re
     text = open(path, 'r', encoding='utf-8').read()
     text = re.sub(r'/\*.*?\*/', ' ', text, flags=re.S)
@@ -52,7 +52,7 @@ def _parse_header(path: str) -> Dict[str, str]:
                 return 'p'
             base = decl.replace('const', ' ').split()
             ty = base[0]
-            return {'int': 'i', 'int32_t': 'i', 'int64_t': 'l', 'float': 'f'}[ty]
+            return {'int': 'i', 'int32_t': 'i', 'int64_t': 'l', 'float': 'f', 'double': 'd'}[ty]
 
         args = '' if params in ('', 'void') else ''.join(code(p) for p in params.split(','))
         sigs[name] = args + '->' + code(ret + ' x' if '*' not in ret else ret, True)
@@ -61,7 +61,7 @@ def _parse_header(path: str) -> Dict[str, str]:
 
 SIGNATURES: Dict[str, str] = _parse_header(header_path())
 
-_CTYPES = {'i': ctypes.c_int, 'l': ctypes.c_int64, 'f': ctypes.c_float, 'p': ctypes.c_void_p,
+_CTYPES = {'i': ctypes.c_int, 'l': ctypes.c_int64, 'f': ctypes.c_float, 'd': ctypes.c_double, 'p': ctypes.c_void_p,
            's': ctypes.c_void_p, 'c': ctypes.c_char_p}
 
 _lib: Optional[ctypes.CDLL] = None

@@ -6,6 +6,7 @@ Restates `tracegnn/models/trace_vae/train.py`:
 * two-phase schedule (all parameters, then `latency_vae.*` only with the rest
   of the model in eval mode), LR annealing from the global epoch                :204-208, 374-383, 455-487
 * clip by global norm 10 + RMSprop / Adam (tensorkit `fit_model`)               :369-372, 417-426
+  (beyond the reference: AdamW, `--train.optimizer=adamw` / `adamw8`)
 * `models/{epoch}.pt`, `models/final.pt` = `torch.save(vae.state_dict())`        :343-352
 
 MI355X-side design: all parameters live in ONE flat fp32 buffer (struct part first, the
@@ -29,6 +30,7 @@ from . import hip, ops
 from .batch import DeviceTraceStore, TraceGraphBatch
 from .config import ExpConfig, config_to_dict
 from .model import TraceVAE
+from .optim import AdamW
 
 __all__ = ['NANLossError', 'FlatParameters', 'FlatOptimizer', 'compute_train_loss', 'Trainer',
            'l2_parameter_names', 'learning_rate_for_epoch', 'save_model', 'StoreStream', 'fit',
@@ -143,15 +145,27 @@ class FlatParameters(object):
 
 class FlatOptimizer(object):
     """RMSprop / Adam over a range of the flat buffer, with clip-by-global-norm
-    (`tv_sumsq_partial` -> `tv_sum_partials` -> `tv_optim_step`)."""
+    (`tv_sumsq_partial` -> `tv_sum_partials` -> `tv_optim_step`); or AdamW over the parameters of
+    that range (`optim.AdamW`: 'adamw' with moments in 32 bits, 'adamw8' in 8), whose weight decay
+    leaves biases out as the L2 term does."""
 
     def __init__(self, flat: FlatParameters, kind: str = 'rmsprop', start: int = 0,
                  end: Optional[int] = None, alpha: float = 0.99, betas=(0.9, 0.999),
-                 eps: float = 1e-8):
+                 eps: float = 1e-8, weight_decay: float = 0.0, seed: int = 0):
         self.flat, self.kind = flat, kind.lower()
-        if self.kind not in ('rmsprop', 'adam'):
+        if self.kind not in ('rmsprop', 'adam', 'adamw', 'adamw8'):
             raise ValueError(f'unknown optimizer {kind!r}')
         self.start, self.end = start, flat.total if end is None else end
+        if self.kind in ('adamw', 'adamw8'):
+            names = [n for n in flat.names if self.start <= flat.slices[n][0] < self.end]
+            self._grads = [flat.grad_views[n] for n in names]
+            self.adamw = AdamW([flat.params[n].data for n in names], betas=betas, eps=eps,
+                               weight_decay=[0.0 if 'bias' in n else weight_decay for n in names],
+                               state_bits=8 if self.kind == 'adamw8' else 32, seed=seed)
+            self.lr = self.adamw.lr
+            self.grad_norm = self.adamw.grad_norm
+            return
+        self.adamw = None
         n = self.end - self.start
         dev = flat.flat.device
         self.state1 = torch.zeros(n, dtype=torch.float32, device=dev)
@@ -164,12 +178,17 @@ class FlatOptimizer(object):
 
     def set_lr(self, lr: float) -> None:
         self.lr = float(lr)
+        if self.adamw is not None:
+            self.adamw.set_lr(self.lr)
 
     def step(self, global_clip_norm: Optional[float], guard: Optional[torch.Tensor] = None,
              guard_kind: int = 0, guard_host: Optional[torch.Tensor] = None) -> None:
         """`guard` (a device scalar): the update is skipped on the device when it is NaN
         (guard_kind 1) or non-zero (guard_kind 2) - `tv_optim_step_guarded`; `guard_host`
         (one pinned host float) receives the scalar from the kernel."""
+        if self.adamw is not None:
+            self.adamw.step(self._grads, global_clip_norm, guard, guard_kind, guard_host)
+            return
         n = self.end - self.start
         p = self.flat.flat[self.start:self.end]
         g = self.flat.grad[self.start:self.end]
@@ -256,7 +275,9 @@ class Trainer(object):
         for n, p in f.params.items():
             p.requires_grad_(n in in_part)
         start = f.tail_start if latency_only else 0
-        self.optimizer = FlatOptimizer(f, self.train_cfg.optimizer, start, f.total)
+        self.optimizer = FlatOptimizer(f, self.train_cfg.optimizer, start, f.total,
+                                       weight_decay=self.train_cfg.weight_decay,
+                                       seed=self.config.seed or 0)
         self.optimizer.set_lr(learning_rate_for_epoch(self.train_cfg, self.epoch - 1))
         self.l2_names = l2_parameter_names(f.all_names, part)
         self.l2_mask = f.mask(self.l2_names)
