@@ -711,7 +711,8 @@ int tv_optim_step_guarded(int kind, int64_t n, float *param, const float *grad, 
  * caller-owned, 16-byte aligned, zero before the first step:
  *   state_bits 32: moment1 = m, moment2 = v, fp32; scales NULL
  *   state_bits  8: moment1 = m / scale1, moment2 = sqrt(v) / scale2, one e4m3 byte each, one fp32
- *     scale per TV_ADAMW_BLOCK elements = (largest finite magnitude of the block) / 448.  Codes are
+ *     scale per TV_ADAMW_BLOCK elements = (largest finite magnitude of the block) * fp32(1/448).  Codes
+ *     are
  *     rounded up or down with the probabilities that keep the value on average, by a hash of
  *     (seed, step, element): same seed, same bits.  A positive sqrt(v) keeps a positive code; an
  *     infinite or NaN moment becomes the NaN code and leaves its neighbours alone; a block whose

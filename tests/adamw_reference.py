@@ -26,7 +26,7 @@ def to_codes(x, random16, positive):
     """(values of e4m3, scales) of `x` [blocks, 256] float64."""
     finite = torch.isfinite(x)
     mag = torch.where(finite, x.abs(), 0.0)
-    scale = mag.amax(1, keepdim=True).float() / 448
+    scale = mag.amax(1, keepdim=True).float() * torch.tensor(1 / 448, dtype=torch.float32)
     scale = torch.where(scale >= 2.0 ** -126, scale, torch.zeros_like(scale))
     y = torch.where(scale > 0, mag / scale.double(), 0.0).clamp(max=448.0)
     at = torch.searchsorted(GRID, y.contiguous(), right=True) - 1

@@ -265,7 +265,7 @@ __device__ __forceinline__ uint32_t code_of(double y, uint32_t random16) {
   return c < 126u ? c : 126u;
 }
 __device__ __forceinline__ float scale_of(float largest) {
-  const float s = largest / 448.f;
+  const float s = largest * (1.f / 448.f);
   return s >= 1.17549435e-38f ? s : 0.f;          // (below that the block counts as zero)
 }
 __device__ __forceinline__ bool finite(double x) {

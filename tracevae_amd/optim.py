@@ -98,7 +98,7 @@ class AdamW(object):
         self._lr = self._control.view(torch.float64)[1]
         self._write_control(0)
         self._workspace = zeros(int(lib.tv_adamw_workspace_bytes(n)) // 8, torch.float64)
-        self.grad_norm = zeros(1, torch.float64)
+        self.grad_norm = torch.zeros((), dtype=torch.float64, device=self.device)
         self._plan_host, self._plan, self._where = None, None, None
         self._make_plan()
 
