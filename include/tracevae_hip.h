@@ -494,6 +494,26 @@ int tv_embedding_fwd(int64_t rows, int64_t dim, int64_t num_operations, const fl
 int tv_embedding_bwd(int64_t rows, int64_t dim, int64_t num_operations, const int64_t *ids,
                      const float *dout, int64_t ld, int64_t col0, float *dweight, void *stream);
 
+/* Rows of a table by token id, times a scale, and the gradient of the table by sorted tokens (the
+ * operation embedding, model/operation_embedding.py:21-25, as tables of many tokens need it):
+ *   out[r]     = round(scale * weight[ids[r]])   rows of zeros for ids outside [0, num_tokens) and
+ *                                                for padding_id (-1: none)
+ *   dweight[v] = round(scale * sum over r with ids[r] = v of dout[r]); every row is written
+ * weight / out types (TV_DTYPE_*): equal, or an fp32 table with 16-bit rows; dout has out's type,
+ * dweight weight's, [num_tokens, dim] dense.  Row strides in elements; no alignment beyond the
+ * type's is needed (rows at multiples of 16 bytes are the fastest).  Sums are fp32 in a fixed
+ * order, rounded once.  rows, num_tokens < 2^31 - 1; dim <= 65536.
+ * Workspace of the backward pass: 16-byte aligned, tv_scaled_embedding_bwd_workspace_bytes. */
+int tv_scaled_embedding_fwd(int64_t rows, int64_t dim, int64_t num_tokens, int weight_dtype,
+                            int out_dtype, const void *weight, int64_t weight_stride,
+                            const int64_t *ids, int64_t padding_id, float scale, void *out,
+                            int64_t out_stride, void *stream);
+int64_t tv_scaled_embedding_bwd_workspace_bytes(int64_t rows, int64_t dim, int64_t num_tokens);
+int tv_scaled_embedding_bwd(int64_t rows, int64_t dim, int64_t num_tokens, int weight_dtype,
+                            int out_dtype, const int64_t *ids, int64_t padding_id, float scale,
+                            const void *dout, int64_t dout_stride, void *dweight, void *workspace,
+                            int64_t workspace_bytes, void *stream);
+
 /* latency-decoder input rows [z2 (broadcast over the M slots) || emb[node_type_pad]]
  * (model/latency_vae.py:320-343): out [K*B*M, Z2+E]; bwd: dz2[k,b,:] = sum_m d(out)[..., :Z2] */
 int tv_latdec_input_fwd(int64_t n_samples, int64_t batch, int64_t max_node_count, int64_t z2_dim,
