@@ -16,83 +16,108 @@
 namespace {
 
 constexpr int TE_THREADS = 256;
-constexpr int TE_ITEMS = 2048;                    // ids per workgroup of a sort pass
+constexpr int TE_SORT_THREADS = 1024;             // of a sort workgroup
+constexpr int TE_SORT_WAVES = TE_SORT_THREADS / 64;
+constexpr int TE_SMALL = 8192;                    // rows that one workgroup sorts alone
+constexpr int TE_SORT_BLOCKS = 64;                // sort workgroups of longer lists, at most
 constexpr int TE_MAX_BITS = 10;                   // of a digit
 constexpr int TE_MAX_BINS = 1 << TE_MAX_BITS;
+constexpr int TE_BATCH = 8;                       // rows whose loads are in flight together
+constexpr int TE_JOIN_THREADS = 1024;
 
-template <int N, typename T> struct Vec {
-  T v[N];
-} __attribute__((packed, aligned(sizeof(T))));
-
-// N consecutive elements as floats; 16 bytes at once, at any alignment of the type
+// N consecutive elements at any alignment of the type, in one access of up to 16 bytes
+template <int N, typename T> struct Some {
+  typedef T V __attribute__((ext_vector_type(N)));
+  typedef V Any __attribute__((aligned(sizeof(T))));
+};
 template <int N, typename T> __device__ __forceinline__ void load_n(const T *p, float (&x)[N]) {
-  const Vec<N, T> f = *reinterpret_cast<const Vec<N, T> *>(p);
+  constexpr int M = N * sizeof(T) > 16 ? 16 / sizeof(T) : N;
+  if constexpr (N == 1) {
+    x[0] = (float)p[0];
+  } else {
 #pragma unroll
-  for (int j = 0; j < N; ++j) x[j] = (float)f.v[j];
+    for (int k = 0; k < N; k += M) {
+      const typename Some<M, T>::V f = *reinterpret_cast<const typename Some<M, T>::Any *>(p + k);
+#pragma unroll
+      for (int j = 0; j < M; ++j) x[k + j] = (float)f[j];
+    }
+  }
 }
 template <int N, typename T> __device__ __forceinline__ void store_n(T *p, const float (&x)[N]) {
-  Vec<N, T> f;
-#pragma unroll
-  for (int j = 0; j < N; ++j) f.v[j] = (T)x[j];
-  *reinterpret_cast<Vec<N, T> *>(p) = f;
-}
-
-// the part of a row that starts at column `col`: N columns, fewer at the end of the row
-template <int N, typename T>
-__device__ __forceinline__ void load_part(const T *row, int64_t col, int64_t dim, float (&x)[N]) {
-  if (col + N <= dim) {
-    load_n<N, T>(row + col, x);
+  constexpr int M = N * sizeof(T) > 16 ? 16 / sizeof(T) : N;
+  if constexpr (N == 1) {
+    p[0] = (T)x[0];
   } else {
 #pragma unroll
-    for (int j = 0; j < N; ++j) x[j] = col + j < dim ? (float)row[col + j] : 0.f;
-  }
-}
-template <int N, typename T>
-__device__ __forceinline__ void store_part(T *row, int64_t col, int64_t dim, const float (&x)[N]) {
-  if (col + N <= dim) {
-    store_n<N, T>(row + col, x);
-  } else {
+    for (int k = 0; k < N; k += M) {
+      typename Some<M, T>::Any f;
 #pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (col + j < dim) row[col + j] = (T)x[j];
+      for (int j = 0; j < M; ++j) f[j] = (T)x[k + j];
+      *reinterpret_cast<typename Some<M, T>::Any *>(p + k) = f;
+    }
   }
 }
 
+// Columns of a row are cut into parts of N; the last part ends with the row and overlaps the one in
+// front of it if N does not divide the row: both hold the same values there, so no part is masked.
+// Rows shorter than N use N = 1.
+__device__ __forceinline__ int64_t part_column(int64_t part, int n, int64_t dim) {
+  const int64_t c = part * n;
+  return c + n <= dim ? c : dim - n;
+}
+
 // ---------------------------------------------------------------------------------------
-// forward
+// forward: 2^lg threads per row, ROWS rows per thread with their loads in flight together
 // ---------------------------------------------------------------------------------------
-template <typename W, typename O, int N>
+template <typename W, typename O, int N, int ROWS>
 __global__ __launch_bounds__(TE_THREADS) void lookup_kernel(int64_t rows, int64_t dim, int64_t vocab,
-                                                            int64_t parts, const W *__restrict__ weight,
+                                                            int parts, int lg, const W *__restrict__ weight,
                                                             int64_t weight_stride,
                                                             const int64_t *__restrict__ ids,
                                                             int64_t padding, float scale,
                                                             O *__restrict__ out, int64_t out_stride) {
-  const int64_t total = rows * parts, stride = (int64_t)gridDim.x * TE_THREADS;
-  for (int64_t e = (int64_t)blockIdx.x * TE_THREADS + threadIdx.x; e < total; e += stride) {
-    const int64_t r = e / parts, col = (e - r * parts) * N;
-    const int64_t id = ids[r];
-    float x[N];
-    if (id >= 0 && id < vocab && id != padding) {
-      load_part<N, W>(weight + id * weight_stride, col, dim, x);
+  const int per = TE_THREADS >> lg;               // rows per workgroup and trip
+  const int64_t r0 = (int64_t)blockIdx.x * per * ROWS + (threadIdx.x >> lg);
+  int64_t id[ROWS];
 #pragma unroll
-      for (int j = 0; j < N; ++j) x[j] *= scale;
-    } else {
+  for (int k = 0; k < ROWS; ++k) {
+    const int64_t r = r0 + (int64_t)k * per;
+    id[k] = r < rows ? ids[r] : -1;
+    if (id[k] >= vocab || id[k] == padding) id[k] = -1;
+  }
+  for (int part = threadIdx.x & ((1 << lg) - 1); part < parts; part += 1 << lg) {
+    const int64_t col = part_column(part, N, dim);
+    float x[ROWS][N];
 #pragma unroll
-      for (int j = 0; j < N; ++j) x[j] = 0.f;
+    for (int k = 0; k < ROWS; ++k) {
+      if (id[k] >= 0) {
+        load_n<N, W>(weight + id[k] * weight_stride + col, x[k]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) x[k][j] = 0.f;
+      }
     }
-    store_part<N, O>(out + r * out_stride, col, dim, x);
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+      const int64_t r = r0 + (int64_t)k * per;
+      if (r >= rows) break;
+      if (id[k] >= 0) {                           // (0 * scale is no zero for an infinite scale)
+#pragma unroll
+        for (int j = 0; j < N; ++j) x[k][j] *= scale;
+      }
+      store_n<N, O>(out + r * out_stride + col, x[k]);
+    }
   }
 }
 
 // ---------------------------------------------------------------------------------------
-// sort: one pass over one digit of the token = histogram, scan, scatter
+// stable counting sort of (token, row) by digits of the token, lowest first
 // ---------------------------------------------------------------------------------------
 // padding and ids outside the table get the token `vocab`, which sorts behind all others
 __device__ __forceinline__ uint32_t token_of(int64_t id, int64_t vocab, int64_t padding) {
   return id >= 0 && id < vocab && id != padding ? (uint32_t)id : (uint32_t)vocab;
 }
-struct Keys {                                     // either the ids themselves or sorted pairs
+struct Keys {                                     // either the ids themselves or pairs of an earlier pass
   const int64_t *ids;
   const uint2 *pairs;
   int64_t vocab, padding;
@@ -101,128 +126,197 @@ struct Keys {                                     // either the ids themselves o
   }
 };
 
-__global__ __launch_bounds__(TE_THREADS) void digit_count_kernel(int64_t n, Keys keys, int shift,
-                                                                 int bins, int64_t nblk,
-                                                                 uint32_t *__restrict__ counts) {
-  __shared__ uint32_t hist[TE_MAX_BINS];
-  for (int b = threadIdx.x; b < bins; b += TE_THREADS) hist[b] = 0;
-  __syncthreads();
-  const int64_t i0 = (int64_t)blockIdx.x * TE_ITEMS;
-  for (int k = threadIdx.x; k < TE_ITEMS; k += TE_THREADS)
-    if (i0 + k < n) atomicAdd(&hist[(keys.at(i0 + k).x >> shift) & (bins - 1)], 1u);
-  __syncthreads();
-  for (int b = threadIdx.x; b < bins; b += TE_THREADS) counts[(int64_t)b * nblk + blockIdx.x] = hist[b];
-}
-
-// per digit: counts -> exclusive sums over the workgroups, the total behind
-__global__ __launch_bounds__(TE_THREADS) void digit_scan_kernel(int bins, int64_t nblk,
-                                                                uint32_t *__restrict__ counts,
-                                                                uint32_t *__restrict__ totals) {
-  const int lane = threadIdx.x & 63;
-  const int b = (int)blockIdx.x * (TE_THREADS / 64) + (threadIdx.x >> 6);
-  if (b >= bins) return;
-  uint32_t *row = counts + (int64_t)b * nblk;
-  uint32_t carry = 0;
-  for (int64_t i0 = 0; i0 < nblk; i0 += 64) {
-    const uint32_t c = i0 + lane < nblk ? row[i0 + lane] : 0u;
-    uint32_t s = c;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const uint32_t t = __shfl_up(s, o, 64);
-      if (lane >= o) s += t;
-    }
-    if (i0 + lane < nblk) row[i0 + lane] = carry + s - c;
-    carry += __shfl(s, 63, 64);
+// lanes of the wave with the same digit (among those that are `in`)
+__device__ __forceinline__ uint64_t same_digit(uint32_t d, bool in, int bits) {
+  uint64_t same = __ballot(in);
+  for (int bit = 0; bit < bits; ++bit) {
+    const uint64_t set = __ballot((d >> bit) & 1u);
+    same &= (d >> bit) & 1u ? set : ~set;
   }
-  if (lane == 0) totals[b] = carry;
+  return same;
+}
+// exclusive sum over the 1024 threads of a sort workgroup
+__device__ __forceinline__ uint32_t sort_exclusive_sum(uint32_t c, uint32_t *wave_sum) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  uint32_t s = c;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t t = __shfl_up(s, o, 64);
+    if (lane >= o) s += t;
+  }
+  if (lane == 63) wave_sum[w] = s;
+  __syncthreads();
+  uint32_t before = s - c;
+  for (int k = 0; k < w; ++k) before += wave_sum[k];
+  __syncthreads();
+  return before;
 }
 
-// stable: wave w of a workgroup takes the w-th quarter of its ids, 64 at a time; equal digits among
-// the 64 are ranked by lane, and a wave's own counter carries the rank from round to round
-__global__ __launch_bounds__(TE_THREADS) void digit_scatter_kernel(
-    int64_t n, Keys keys, int shift, int bits, int64_t nblk, const uint32_t *__restrict__ counts,
-    const uint32_t *__restrict__ totals, uint2 *__restrict__ out) {
-  constexpr int WAVES = TE_THREADS / 64, ROUNDS = TE_ITEMS / TE_THREADS;
-  __shared__ uint32_t seen[WAVES][TE_MAX_BINS];
-  __shared__ uint32_t first[TE_MAX_BINS];
-  __shared__ uint32_t wave_sum[WAVES];
+// Up to TE_SMALL rows: all passes in one workgroup, the pairs in LDS between them.  Wave w takes the
+// w-th run of 64 * ROUNDS pairs; equal digits among 64 are ranked by lane, and the wave's own counter
+// carries the rank from round to round.
+template <int ROUNDS>
+__global__ __launch_bounds__(TE_SORT_THREADS) void small_sort_kernel(int n, Keys keys, int bits, int passes,
+                                                                     uint2 *__restrict__ out) {
+  __shared__ uint32_t seen[TE_SORT_WAVES][TE_MAX_BINS];
+  __shared__ uint32_t wave_sum[TE_SORT_WAVES];
+  __shared__ uint2 pairs[ROUNDS * TE_SORT_THREADS];
   const int bins = 1 << bits, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  for (int b = lane; b < bins; b += 64) seen[w][b] = 0;
-  // first place of each digit: exclusive sums of the totals (4 digits per thread)
-  {
-    uint32_t c[TE_MAX_BINS / TE_THREADS], sum = 0;
-#pragma unroll
-    for (int k = 0; k < TE_MAX_BINS / TE_THREADS; ++k) {
-      const int b = (int)threadIdx.x * (TE_MAX_BINS / TE_THREADS) + k;
-      c[k] = b < bins ? totals[b] : 0u;
-      sum += c[k];
-    }
-    uint32_t s = sum;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const uint32_t t = __shfl_up(s, o, 64);
-      if (lane >= o) s += t;
-    }
-    if (lane == 63) wave_sum[w] = s;
-    __syncthreads();
-    uint32_t before = s - sum;
-    for (int k = 0; k < w; ++k) before += wave_sum[k];
-#pragma unroll
-    for (int k = 0; k < TE_MAX_BINS / TE_THREADS; ++k) {
-      const int b = (int)threadIdx.x * (TE_MAX_BINS / TE_THREADS) + k;
-      if (b < bins) first[b] = before + counts[(int64_t)b * nblk + blockIdx.x];
-      before += c[k];
-    }
-  }
-  __syncthreads();
-  const int64_t i0 = (int64_t)blockIdx.x * TE_ITEMS + (int64_t)w * (TE_ITEMS / WAVES);
+  const int i0 = w * 64 * ROUNDS + lane;
   uint2 item[ROUNDS];
-  uint32_t rank[ROUNDS];
 #pragma unroll
-  for (int k = 0; k < ROUNDS; ++k) {
-    const int64_t i = i0 + k * 64 + lane;
-    const bool in = i < n;
-    item[k] = in ? keys.at(i) : make_uint2(0u, 0u);
-    const uint32_t d = (item[k].x >> shift) & (bins - 1);
-    uint64_t same = __ballot(in);
-    for (int bit = 0; bit < bits; ++bit) {
-      const uint64_t set = __ballot((d >> bit) & 1u);
-      same &= (d >> bit) & 1u ? set : ~set;
+  for (int k = 0; k < ROUNDS; ++k) item[k] = i0 + k * 64 < n ? keys.at(i0 + k * 64) : make_uint2(0u, 0u);
+  for (int p = 0; p < passes; ++p) {
+    const int shift = p * bits;
+    for (int b = lane; b < bins; b += 64) seen[w][b] = 0;
+    uint32_t rank[ROUNDS];
+#pragma unroll
+    for (int k = 0; k < ROUNDS; ++k) {
+      const bool in = i0 + k * 64 < n;
+      const uint32_t d = (item[k].x >> shift) & (bins - 1);
+      const uint64_t same = same_digit(d, in, bits);
+      const uint32_t below = (uint32_t)__popcll(same & ((1ull << lane) - 1ull));
+      // (LDS accesses of one wave stay in order; the fences keep the compiler from moving them)
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      rank[k] = in ? seen[w][d] + below : 0u;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      if (in && below == 0) seen[w][d] += (uint32_t)__popcll(same);
     }
-    const uint32_t below = (uint32_t)__popcll(same & ((1ull << lane) - 1ull));
-    rank[k] = 0;
-    if (in) rank[k] = seen[w][d] + below;
-    // (LDS accesses of one wave stay in order; the fences keep the compiler from moving them)
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    if (in && below == 0) seen[w][d] += (uint32_t)__popcll(same);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  }
-  __syncthreads();
-  // where each wave's run of a digit begins
-  for (int b = threadIdx.x; b < bins; b += TE_THREADS) {
-    uint32_t at = first[b];
+    __syncthreads();
+    // counts -> first places: digits in order, within a digit the waves in order
+    uint32_t total = 0;
+    const int b = threadIdx.x;
+    if (b < bins) {
 #pragma unroll
-    for (int k = 0; k < WAVES; ++k) {
+      for (int k = 0; k < TE_SORT_WAVES; ++k) {
+        const uint32_t c = seen[k][b];
+        seen[k][b] = total;
+        total += c;
+      }
+    }
+    const uint32_t first = sort_exclusive_sum(b < bins ? total : 0u, wave_sum);
+    if (b < bins) {
+#pragma unroll
+      for (int k = 0; k < TE_SORT_WAVES; ++k) seen[k][b] += first;
+    }
+    __syncthreads();
+    uint2 *to = p + 1 < passes ? pairs : out;
+#pragma unroll
+    for (int k = 0; k < ROUNDS; ++k)
+      if (i0 + k * 64 < n) to[seen[w][(item[k].x >> shift) & (bins - 1)] + rank[k]] = item[k];
+    if (p + 1 < passes) {
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < ROUNDS; ++k)
+        if (i0 + k * 64 < n) item[k] = pairs[i0 + k * 64];
+    }
+  }
+}
+
+// Longer lists: every workgroup takes one run of `items` (a multiple of 64 * TE_SORT_WAVES) pairs.
+__global__ __launch_bounds__(TE_SORT_THREADS) void digit_count_kernel(int64_t n, Keys keys, int shift,
+                                                                      int bits, int64_t items,
+                                                                      uint32_t *__restrict__ counts) {
+  __shared__ uint32_t hist[TE_MAX_BINS];
+  const int bins = 1 << bits;
+  if ((int)threadIdx.x < bins) hist[threadIdx.x] = 0;
+  __syncthreads();
+  const int64_t i0 = (int64_t)blockIdx.x * items, i1 = i0 + items < n ? i0 + items : n;
+#pragma unroll 4
+  for (int64_t i = i0 + threadIdx.x; i < i1; i += TE_SORT_THREADS)
+    atomicAdd(&hist[(keys.at(i).x >> shift) & (bins - 1)], 1u);
+  __syncthreads();
+  if ((int)threadIdx.x < bins) counts[(int64_t)blockIdx.x * bins + threadIdx.x] = hist[threadIdx.x];
+}
+
+__global__ __launch_bounds__(TE_SORT_THREADS) void digit_scatter_kernel(
+    int64_t n, Keys keys, int shift, int bits, int64_t items, int nblk,
+    const uint32_t *__restrict__ counts, uint2 *__restrict__ out) {
+  __shared__ uint32_t seen[TE_SORT_WAVES][TE_MAX_BINS];
+  __shared__ uint32_t wave_sum[TE_SORT_WAVES];
+  const int bins = 1 << bits, lane = threadIdx.x & 63, w = threadIdx.x >> 6, b = threadIdx.x;
+  for (int k = lane; k < bins; k += 64) seen[w][k] = 0;
+  // the digit's pairs in the workgroups before this one, and in all
+  uint32_t before = 0, total = 0;
+  if (b < bins) {
+#pragma unroll 16
+    for (int k = 0; k < nblk; ++k) {
+      const uint32_t c = counts[(int64_t)k * bins + b];
+      before += k < (int)blockIdx.x ? c : 0u;
+      total += c;
+    }
+  }
+  const int64_t run = items / TE_SORT_WAVES;
+  const int64_t i0 = (int64_t)blockIdx.x * items + w * run;
+  const int64_t i1 = i0 + run < n ? i0 + run : n;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll 4
+  for (int64_t i = i0 + lane; i < i1; i += 64)
+    atomicAdd(&seen[w][(keys.at(i).x >> shift) & (bins - 1)], 1u);
+  __syncthreads();
+  uint32_t at = sort_exclusive_sum(b < bins ? total : 0u, wave_sum) + before;
+  if (b < bins) {
+#pragma unroll
+    for (int k = 0; k < TE_SORT_WAVES; ++k) {
       const uint32_t c = seen[k][b];
       seen[k][b] = at;
       at += c;
     }
   }
   __syncthreads();
-#pragma unroll
-  for (int k = 0; k < ROUNDS; ++k) {
-    const int64_t i = i0 + k * 64 + lane;
-    if (i < n) out[seen[w][(item[k].x >> shift) & (bins - 1)] + rank[k]] = item[k];
+  for (int64_t j = i0; j < i1; j += 64) {
+    const int64_t i = j + lane;
+    const bool in = i < i1;
+    const uint2 item = in ? keys.at(i) : make_uint2(0u, 0u);
+    const uint32_t d = (item.x >> shift) & (bins - 1);
+    const uint64_t same = same_digit(d, in, bits);
+    const uint32_t below = (uint32_t)__popcll(same & ((1ull << lane) - 1ull));
+    // (LDS accesses of one wave stay in order; the fences keep the compiler from moving them)
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const uint32_t to = in ? seen[w][d] + below : 0u;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (in && below == 0) seen[w][d] += (uint32_t)__popcll(same);
+    if (in) out[to] = item;
   }
 }
 
 // ---------------------------------------------------------------------------------------
 // sums over the sorted list
 // ---------------------------------------------------------------------------------------
-template <typename T>
-__global__ __launch_bounds__(TE_THREADS) void zero_rows_kernel(int64_t n, T *__restrict__ x) {
-  const int64_t stride = (int64_t)gridDim.x * TE_THREADS;
-  for (int64_t i = (int64_t)blockIdx.x * TE_THREADS + threadIdx.x; i < n; i += stride) x[i] = (T)0.f;
+// rows of dW that no token names, 16 per wave: a binary search in the sorted list for each
+template <typename W>
+__device__ __forceinline__ void zero_absent_rows(int64_t wave, int64_t n, int64_t dim, int64_t vocab,
+                                                 const uint2 *__restrict__ sorted, W *__restrict__ dweight) {
+  const int lane = threadIdx.x & 63;
+  const int64_t v0 = wave * 16, v = v0 + lane;
+  bool absent = false;
+  if (lane < 16 && v < vocab) {
+    int64_t lo = 0, hi = n;                       // the first pair whose token is not below v
+    while (lo < hi) {
+      const int64_t mid = (lo + hi) >> 1;
+      if ((int64_t)sorted[mid].x < v) lo = mid + 1;
+      else hi = mid;
+    }
+    absent = lo >= n || (int64_t)sorted[lo].x != v;
+  }
+  uint64_t rows = __ballot(absent);
+  while (rows) {
+    const int bit = __builtin_ctzll(rows);
+    rows &= rows - 1;
+    W *row = dweight + (v0 + bit) * dim;
+    constexpr int M = 16 / sizeof(W);
+    if (dim >= M) {
+      const int64_t parts = (dim + M - 1) / M;
+      for (int64_t part = lane; part < parts; part += 64) {
+        float zero[M];
+#pragma unroll
+        for (int j = 0; j < M; ++j) zero[j] = 0.f;
+        store_n<M, W>(row + part_column(part, M, dim), zero);
+      }
+    } else if (lane < dim) {
+      row[lane] = (W)0.f;
+    }
+  }
 }
 
 // A group of G lanes, N columns each, walks one tile.  A token that neither begins before the tile
@@ -230,102 +324,215 @@ __global__ __launch_bounds__(TE_THREADS) void zero_rows_kernel(int64_t n, T *__r
 // tile, of one that begins here and goes on to slot 1.
 template <typename D, typename W, int N, int G>
 __global__ __launch_bounds__(TE_THREADS) void tile_sums_kernel(
-    int64_t n, int64_t dim, int64_t vocab, int tile, int64_t tiles, int64_t slabs,
+    int64_t n, int64_t dim, int64_t vocab, int tile, int64_t tiles, int64_t slabs, int64_t tile_blocks,
     const uint2 *__restrict__ sorted, const D *__restrict__ dout, int64_t dout_stride, float scale,
     W *__restrict__ dweight, float *__restrict__ part) {
-  const int64_t unit = ((int64_t)blockIdx.x * TE_THREADS + threadIdx.x) / G;
-  const int lane = threadIdx.x % G;
+  if ((int64_t)blockIdx.x >= tile_blocks) {
+    zero_absent_rows<W>(((int64_t)blockIdx.x - tile_blocks) * (TE_THREADS / 64) + (threadIdx.x >> 6), n, dim,
+                        vocab, sorted, dweight);
+    return;
+  }
+  const int64_t unit = (int64_t)blockIdx.x * (TE_THREADS / G) + threadIdx.x / G;
   if (unit >= tiles * slabs) return;
-  const int64_t t = unit / slabs, col = ((unit - t * slabs) * G + lane) * N;
+  const int64_t t = unit / slabs, column_part = (unit - t * slabs) * G + threadIdx.x % G;
+  const bool active = column_part * N < dim;
+  const int64_t col = active ? part_column(column_part, N, dim) : 0;
   const int64_t i0 = t * tile, i1 = i0 + tile < n ? i0 + tile : n;
   uint32_t cur = sorted[i0].x;
   if (cur >= vocab) return;                       // nothing but padding from here on
   bool began_before = i0 > 0 && sorted[i0 - 1].x == cur;
+  const uint32_t behind = i1 < n ? sorted[i1].x : 0xffffffffu;
   float acc[N];
 #pragma unroll
   for (int j = 0; j < N; ++j) acc[j] = 0.f;
   auto write = [&](bool goes_on) {
-    if (began_before || goes_on) {
-      if (col < dim) store_part<N, float>(part + (t * 2 + (began_before ? 0 : 1)) * dim, col, dim, acc);
-    } else {
-      float y[N];
+    if (active) {
+      if (began_before || goes_on) {
+        store_n<N, float>(part + (t * 2 + (began_before ? 0 : 1)) * dim + col, acc);
+      } else {
+        float y[N];
 #pragma unroll
-      for (int j = 0; j < N; ++j) y[j] = acc[j] * scale;
-      if (col < dim) store_part<N, W>(dweight + (int64_t)cur * dim, col, dim, y);
+        for (int j = 0; j < N; ++j) y[j] = acc[j] * scale;
+        store_n<N, W>(dweight + (int64_t)cur * dim + col, y);
+      }
     }
 #pragma unroll
     for (int j = 0; j < N; ++j) acc[j] = 0.f;
     began_before = false;
   };
-  for (int64_t i = i0; i < i1; ++i) {
-    const uint2 p = sorted[i];
-    if (p.x != cur) {
-      write(false);
-      cur = p.x;
-      if (cur >= vocab) return;
-    }
-    float x[N];
-    if (col < dim) {
-      load_part<N, D>(dout + (int64_t)p.y * dout_stride, col, dim, x);
+  uint2 next[TE_BATCH];
 #pragma unroll
-      for (int j = 0; j < N; ++j) acc[j] += x[j];
+  for (int k = 0; k < TE_BATCH; ++k) next[k] = sorted[i0 + k < i1 ? i0 + k : i1 - 1];
+  for (int64_t i = i0; i < i1; i += TE_BATCH) {
+    uint2 p[TE_BATCH];
+    float x[TE_BATCH][N];
+#pragma unroll
+    for (int k = 0; k < TE_BATCH; ++k) p[k] = next[k];
+#pragma unroll
+    for (int k = 0; k < TE_BATCH; ++k)            // (rows of padding are inside dout as well)
+      load_n<N, D>(dout + (int64_t)p[k].y * dout_stride + col, x[k]);
+#pragma unroll
+    for (int k = 0; k < TE_BATCH; ++k) {          // the next pairs, on their way behind these rows
+      const int64_t q = i + TE_BATCH + k;
+      next[k] = sorted[q < i1 ? q : i1 - 1];
+    }
+#pragma unroll
+    for (int k = 0; k < TE_BATCH; ++k) {
+      if (i + k >= i1) break;
+      if (p[k].x != cur) {
+        write(false);
+        cur = p[k].x;
+        if (cur >= vocab) return;
+      }
+#pragma unroll
+      for (int j = 0; j < N; ++j) acc[j] += x[k][j];
     }
   }
-  write(i1 < n && sorted[i1].x == cur);
+  write(behind == cur);
 }
 
-// the token that begins in tile t and goes on behind it: its slot there, then slot 0 of the tiles
-// that follow, in order
+// The token that begins in tile t and goes on behind it: its slot there, then slot 0 of the tiles
+// that follow, in order.  A group of G lanes takes the tokens of one tile; a token of more than G
+// tiles is left to the whole workgroup, whose groups take one run of its tiles each.
 template <typename W, int N, int G>
-__global__ __launch_bounds__(TE_THREADS) void join_kernel(int64_t n, int64_t dim, int64_t vocab, int tile,
-                                                          int64_t tiles, int64_t slabs,
-                                                          const uint2 *__restrict__ sorted, float scale,
-                                                          W *__restrict__ dweight,
-                                                          const float *__restrict__ part) {
-  const int64_t unit = ((int64_t)blockIdx.x * TE_THREADS + threadIdx.x) / G;
-  const int lane = threadIdx.x % G;
-  if (unit >= tiles * slabs) return;
-  const int64_t t = unit / slabs, col = ((unit - t * slabs) * G + lane) * N;
+__global__ __launch_bounds__(TE_JOIN_THREADS) void join_kernel(int64_t n, int64_t dim, int64_t vocab, int tile,
+                                                               int64_t tiles, int64_t slabs,
+                                                               const uint2 *__restrict__ sorted, float scale,
+                                                               W *__restrict__ dweight,
+                                                               const float *__restrict__ part) {
+  constexpr int GROUPS = TE_JOIN_THREADS / G;
+  __shared__ int64_t long_end[GROUPS];            // the tile behind the last one of a long token, or 0
+  __shared__ float sums[GROUPS][G * N];
+  const int group = threadIdx.x / G, lane = threadIdx.x % G;
+  auto tile_of = [&](int g, int64_t &t, int64_t &col) -> bool {
+    const int64_t unit = (int64_t)blockIdx.x * GROUPS + g;
+    t = unit / slabs;
+    const int64_t column_part = (unit - t * slabs) * G + lane;
+    const bool active = column_part * N < dim;
+    col = active ? part_column(column_part, N, dim) : 0;
+    return active;
+  };
+  // acc += slot 0 of the tiles u0 .. u1 - 1, in order
+  auto add = [&](int64_t u0, int64_t u1, int64_t col, float (&acc)[N]) {
+    for (int64_t u = u0; u < u1; u += TE_BATCH) {
+      float x[TE_BATCH][N];
+#pragma unroll
+      for (int k = 0; k < TE_BATCH; ++k)
+        load_n<N, float>(part + (u + k < u1 ? u + k : u1 - 1) * 2 * dim + col, x[k]);
+#pragma unroll
+      for (int k = 0; k < TE_BATCH; ++k) {
+        if (u + k >= u1) break;
+#pragma unroll
+        for (int j = 0; j < N; ++j) acc[j] += x[k][j];
+      }
+    }
+  };
+  int64_t t, col;
+  const bool active = tile_of(group, t, col);
+  int64_t end = 0;
+  if (lane == 0) long_end[group] = 0;
   const int64_t i0 = t * tile, i1 = i0 + tile;
-  if (i1 >= n || col >= dim) return;
-  const uint32_t cur = sorted[i1 - 1].x;
-  if (cur >= vocab || sorted[i1].x != cur) return;
-  if (sorted[i0].x == cur && i0 > 0 && sorted[i0 - 1].x == cur) return;     // began before
-  float acc[N];
-  load_part<N, float>(part + (t * 2 + 1) * dim, col, dim, acc);
-  for (int64_t u = t + 1; u < tiles && sorted[u * tile].x == cur; ++u) {
-    float x[N];
-    load_part<N, float>(part + u * 2 * dim, col, dim, x);
+  if (t < tiles && i1 < n) {
+    const uint32_t cur = sorted[i1 - 1].x;
+    const uint32_t next = sorted[i1].x, head = sorted[i0].x, prev = sorted[i0 > 0 ? i0 - 1 : 0].x;
+    if (cur < vocab && next == cur && !(head == cur && i0 > 0 && prev == cur)) {
+      int64_t lo = t + 1, hi = tiles;             // the first tile that does not begin with the token
+      // (the next G tiles at once: a token seldom has more)
+      const int64_t probe = t + 1 + lane;
+      const bool in = probe < tiles && sorted[probe * tile].x == cur;
+      const uint64_t all = __ballot(in);
+      const uint64_t mine = (G == 64 ? all : (all >> ((threadIdx.x & 63) & ~(G - 1)))) & (G == 64 ? ~0ull : ((1ull << (G & 63)) - 1ull));
+      const int run = __popcll(mine);
+      if (run < G) {
+        end = t + 1 + run;
+        float acc[N];
+        load_n<N, float>(part + (t * 2 + 1) * dim + col, acc);
+        add(t + 1, end, col, acc);
 #pragma unroll
-    for (int j = 0; j < N; ++j) acc[j] += x[j];
+        for (int j = 0; j < N; ++j) acc[j] *= scale;
+        if (active) store_n<N, W>(dweight + (int64_t)cur * dim + col, acc);
+      } else {
+        lo = t + 1 + G;
+        while (lo < hi) {
+          const int64_t mid = (lo + hi) >> 1;
+          if (sorted[mid * tile].x == cur) lo = mid + 1;
+          else hi = mid;
+        }
+        if (lane == 0) long_end[group] = lo;
+      }
+    }
   }
+  __syncthreads();
+  for (int g = 0; g < GROUPS; ++g) {
+    const int64_t to = long_end[g];
+    if (to == 0) continue;
+    const bool on = tile_of(g, t, col);
+    const int64_t count = to - (t + 1), each = (count + GROUPS - 1) / GROUPS;
+    const int64_t u0 = t + 1 + group * each < to ? t + 1 + group * each : to;
+    const int64_t u1 = u0 + each < to ? u0 + each : to;
+    float acc[N];
 #pragma unroll
-  for (int j = 0; j < N; ++j) acc[j] *= scale;
-  store_part<N, W>(dweight + (int64_t)cur * dim, col, dim, acc);
+    for (int j = 0; j < N; ++j) acc[j] = 0.f;
+    if (group == 0) load_n<N, float>(part + (t * 2 + 1) * dim + col, acc);
+    add(u0, u1, col, acc);
+#pragma unroll
+    for (int j = 0; j < N; ++j) sums[group][j * G + lane] = acc[j];
+    __syncthreads();
+    if (group == 0) {
+      for (int k = 1; k < GROUPS; ++k)
+#pragma unroll
+        for (int j = 0; j < N; ++j) acc[j] += sums[k][j * G + lane];
+#pragma unroll
+      for (int j = 0; j < N; ++j) acc[j] *= scale;
+      if (on) store_n<N, W>(dweight + (int64_t)sorted[(t + 1) * tile].x * dim + col, acc);
+    }
+    __syncthreads();
+  }
+}
+
+template <typename W>
+__global__ __launch_bounds__(TE_THREADS) void zero_table_kernel(int64_t n, W *__restrict__ dweight) {
+  const int64_t stride = (int64_t)gridDim.x * TE_THREADS;
+  for (int64_t i = (int64_t)blockIdx.x * TE_THREADS + threadIdx.x; i < n; i += stride) dweight[i] = (W)0.f;
 }
 
 // ---------------------------------------------------------------------------------------
 struct Shape {
-  int64_t nblk, tile, tiles;
-  int passes, bits;
-  int64_t pairs0, pairs1, counts, totals, part, bytes;
+  int64_t items, tile, tiles;
+  int nblk, passes, bits;
+  int64_t pairs0, pairs1, counts, part, bytes;
 };
+constexpr int64_t TE_MAX_BLOCKS = ((int64_t)1 << 32) / TE_JOIN_THREADS - 1;     // 2^32 threads per launch
 inline int64_t align256(int64_t x) { return (x + 255) & ~(int64_t)255; }
+
+// lanes of one row: groups of 16, 32 or 64
+inline int64_t lanes_of(int64_t dim, int64_t n) {
+  const int64_t parts = dim < n ? dim : tv_cdiv(dim, n);
+  return parts <= 16 ? 16 : parts <= 32 ? 32 : tv_cdiv(parts, 64) * 64;
+}
 
 inline Shape shape_of(int64_t rows, int64_t dim, int64_t vocab) {
   Shape s = {};
-  s.nblk = tv_cdiv(rows, TE_ITEMS);
+  const int64_t slots = lanes_of(dim, 8);
   int bits = 1;
   while (bits < 32 && ((int64_t)1 << bits) < vocab + 1) ++bits;
   s.passes = (int)tv_cdiv(bits, TE_MAX_BITS);
   s.bits = (int)tv_cdiv(bits, s.passes);
-  s.tile = 32;
+  // one run of ids per sort workgroup
+  s.items = tv_cdiv(tv_cdiv(rows, TE_SORT_BLOCKS), TE_SORT_THREADS) * TE_SORT_THREADS;
+  s.nblk = (int)tv_cdiv(rows, s.items > 0 ? s.items : 1);
+  // Rows per tile: the longest that leaves 1024 waves (four per CU), between 8 and 128.  Longer tiles
+  // leave fewer sums to join, shorter ones more rows in flight: 32768 rows of 1024 bf16 in tiles of 16,
+  // 64 and 128 take 55 + 17, 58 + 12 and 74 + 8 us (tiles + join), 1021 rows of 251 fp16 in tiles of 8 and
+  // 32 take 5.2 + 5.2 and 11.8 + 4.3, 262144 of 512 bf16 in 64 and 128 take 83 + 22 and 83 + 16.
+  s.tile = 8;
+  while (s.tile < 128 && rows * slots / (s.tile * 2) >= 1024 * 64) s.tile *= 2;
   s.tiles = tv_cdiv(rows, s.tile);
+  const bool small = rows <= TE_SMALL;
   s.pairs0 = 0;
   s.pairs1 = align256(rows * 8);
-  s.counts = s.pairs1 + (s.passes > 1 ? align256(rows * 8) : 0);
-  s.totals = s.counts + align256(s.nblk * ((int64_t)4 << s.bits));
-  s.part = s.totals + align256((int64_t)4 << s.bits);
+  s.counts = s.pairs1 + (s.passes > 1 && !small ? align256(rows * 8) : 0);
+  s.part = s.counts + (small ? 0 : align256(s.nblk * ((int64_t)4 << s.bits)));
   s.bytes = s.part + align256(s.tiles * 2 * dim * 4);
   return s;
 }
@@ -335,31 +542,81 @@ inline bool sizes_ok(int64_t rows, int64_t dim, int64_t vocab) {
   return rows >= 0 && rows < INT32_MAX && dim >= 1 && dim <= (1 << 16) && vocab >= 1 && vocab < INT32_MAX;
 }
 
+template <typename W, typename O, int N>
+void launch_lookup_n(int64_t rows, int64_t dim, int64_t vocab, const void *weight, int64_t weight_stride,
+                     const int64_t *ids, int64_t padding, float scale, void *out, int64_t out_stride,
+                     hipStream_t stream) {
+  const int parts = (int)tv_cdiv(dim, N);
+  int lg = 0;
+  while ((1 << lg) < parts && lg < 8) ++lg;
+  const int64_t per = TE_THREADS >> lg;
+  if (tv_cdiv(rows, per) >= 4096)
+    hipLaunchKernelGGL((lookup_kernel<W, O, N, 4>), dim3((unsigned)tv_cdiv(rows, per * 4)), dim3(TE_THREADS), 0,
+                       stream, rows, dim, vocab, parts, lg, (const W *)weight, weight_stride, ids, padding, scale,
+                       (O *)out, out_stride);
+  else
+    hipLaunchKernelGGL((lookup_kernel<W, O, N, 1>), dim3((unsigned)tv_cdiv(rows, per)), dim3(TE_THREADS), 0,
+                       stream, rows, dim, vocab, parts, lg, (const W *)weight, weight_stride, ids, padding, scale,
+                       (O *)out, out_stride);
+}
 template <typename W, typename O>
 void launch_lookup(int64_t rows, int64_t dim, int64_t vocab, const void *weight, int64_t weight_stride,
                    const int64_t *ids, int64_t padding, float scale, void *out, int64_t out_stride,
                    hipStream_t stream) {
-  constexpr int N = 16 / (sizeof(W) < sizeof(O) ? sizeof(O) : sizeof(W));
-  const int64_t parts = tv_cdiv(dim, N);
-  int64_t blocks = tv_cdiv(rows * parts, TE_THREADS);
-  if (blocks > 16384) blocks = 16384;
-  hipLaunchKernelGGL((lookup_kernel<W, O, N>), dim3((unsigned)blocks), dim3(TE_THREADS), 0, stream, rows,
-                     dim, vocab, parts, (const W *)weight, weight_stride, ids, padding, scale, (O *)out,
-                     out_stride);
+  constexpr int N = 16 / sizeof(O);
+  if (dim >= N)
+    launch_lookup_n<W, O, N>(rows, dim, vocab, weight, weight_stride, ids, padding, scale, out, out_stride, stream);
+  else
+    launch_lookup_n<W, O, 1>(rows, dim, vocab, weight, weight_stride, ids, padding, scale, out, out_stride, stream);
 }
 
+void launch_sort(const Shape &s, int64_t rows, Keys keys, char *ws, hipStream_t stream) {
+  uint2 *pairs[2] = {(uint2 *)(ws + s.pairs0), (uint2 *)(ws + s.pairs1)};
+  if (rows <= TE_SMALL) {
+    const int rounds = (int)tv_cdiv(rows, TE_SORT_THREADS);
+    auto kernel = rounds <= 1 ? small_sort_kernel<1> : rounds <= 2 ? small_sort_kernel<2>
+                : rounds <= 4 ? small_sort_kernel<4> : small_sort_kernel<8>;
+    hipLaunchKernelGGL(kernel, dim3(1), dim3(TE_SORT_THREADS), 0, stream, (int)rows, keys, s.bits, s.passes, pairs[0]);
+    return;
+  }
+  uint32_t *counts = (uint32_t *)(ws + s.counts);
+  for (int p = 0; p < s.passes; ++p) {
+    uint2 *to = pairs[(s.passes - 1 - p) & 1];    // (the last pass writes pairs[0])
+    hipLaunchKernelGGL(digit_count_kernel, dim3((unsigned)s.nblk), dim3(TE_SORT_THREADS), 0, stream, rows, keys,
+                       p * s.bits, s.bits, s.items, counts);
+    hipLaunchKernelGGL(digit_scatter_kernel, dim3((unsigned)s.nblk), dim3(TE_SORT_THREADS), 0, stream, rows, keys,
+                       p * s.bits, s.bits, s.items, s.nblk, counts, to);
+    keys.pairs = to;
+  }
+}
+
+template <typename D, typename W, int N, int G>
+void launch_sums_ng(const Shape &s, int64_t rows, int64_t dim, int64_t vocab, const uint2 *sorted,
+                    const void *dout, int64_t dout_stride, float scale, void *dweight, float *part,
+                    hipStream_t stream) {
+  const int64_t slabs = tv_cdiv(tv_cdiv(dim, N), G), units = s.tiles * slabs;
+  const int64_t tile_blocks = tv_cdiv(units, TE_THREADS / G), zero_blocks = tv_cdiv(vocab, 16 * (TE_THREADS / 64));
+  hipLaunchKernelGGL((tile_sums_kernel<D, W, N, G>), dim3((unsigned)(tile_blocks + zero_blocks)), dim3(TE_THREADS),
+                     0, stream, rows, dim, vocab, (int)s.tile, s.tiles, slabs, tile_blocks, sorted,
+                     (const D *)dout, dout_stride, scale, (W *)dweight, part);
+  if (s.tiles > 1)
+    hipLaunchKernelGGL((join_kernel<W, N, G>), dim3((unsigned)tv_cdiv(units, TE_JOIN_THREADS / G)),
+                       dim3(TE_JOIN_THREADS), 0, stream, rows, dim, vocab, (int)s.tile, s.tiles, slabs, sorted,
+                       scale, (W *)dweight, part);
+}
 template <typename D, typename W>
 void launch_sums(const Shape &s, int64_t rows, int64_t dim, int64_t vocab, const uint2 *sorted,
                  const void *dout, int64_t dout_stride, float scale, void *dweight, float *part,
                  hipStream_t stream) {
-  constexpr int N = 16 / sizeof(D), G = 64;
-  const int64_t slabs = tv_cdiv(dim, N * G);
-  const unsigned blocks = (unsigned)tv_cdiv(s.tiles * slabs * G, TE_THREADS);
-  hipLaunchKernelGGL((tile_sums_kernel<D, W, N, G>), dim3(blocks), dim3(TE_THREADS), 0, stream, rows, dim,
-                     vocab, (int)s.tile, s.tiles, slabs, sorted, (const D *)dout, dout_stride, scale,
-                     (W *)dweight, part);
-  hipLaunchKernelGGL((join_kernel<W, N, G>), dim3(blocks), dim3(TE_THREADS), 0, stream, rows, dim, vocab,
-                     (int)s.tile, s.tiles, slabs, sorted, scale, (W *)dweight, part);
+  constexpr int N = 16 / sizeof(D);
+#define TE_NG(n, g) \
+  launch_sums_ng<D, W, n, g>(s, rows, dim, vocab, sorted, dout, dout_stride, scale, dweight, part, stream)
+  const int64_t parts = tv_cdiv(dim, N);
+  if (dim < N) TE_NG(1, 16);
+  else if (parts <= 16) TE_NG(N, 16);
+  else if (parts <= 32) TE_NG(N, 32);
+  else TE_NG(N, 64);
+#undef TE_NG
 }
 
 // (table, rows) types: equal, or an fp32 table with 16-bit rows
@@ -424,37 +681,25 @@ extern "C" int tv_scaled_embedding_bwd(int64_t rows, int64_t dim, int64_t num_to
       return TV_ERR_WORKSPACE;
     }
   }
-  {
+  if (rows == 0) {
     const int64_t count = num_tokens * dim;
     int64_t blocks = tv_cdiv(count, TE_THREADS * 8);
     if (blocks > 16384) blocks = 16384;
     if (weight_dtype == TV_DTYPE_F32)
-      hipLaunchKernelGGL(zero_rows_kernel<float>, dim3((unsigned)blocks), dim3(TE_THREADS), 0, st, count,
+      hipLaunchKernelGGL(zero_table_kernel<float>, dim3((unsigned)blocks), dim3(TE_THREADS), 0, st, count,
                          (float *)dweight);
     else
-      hipLaunchKernelGGL(zero_rows_kernel<_Float16>, dim3((unsigned)blocks), dim3(TE_THREADS), 0, st, count,
+      hipLaunchKernelGGL(zero_table_kernel<_Float16>, dim3((unsigned)blocks), dim3(TE_THREADS), 0, st, count,
                          (_Float16 *)dweight);
     TV_LAUNCH_CHECK("tv_scaled_embedding_bwd");
+    return TV_OK;
   }
-  if (rows == 0) return TV_OK;
   char *ws = (char *)workspace;
-  uint2 *pairs[2] = {(uint2 *)(ws + s.pairs0), (uint2 *)(ws + s.pairs1)};
-  uint32_t *counts = (uint32_t *)(ws + s.counts), *totals = (uint32_t *)(ws + s.totals);
-  Keys keys = {ids, nullptr, num_tokens, padding_id};
-  for (int p = 0; p < s.passes; ++p) {
-    uint2 *to = pairs[(s.passes - 1 - p) & 1];    // (the last pass writes pairs[0])
-    const int bins = 1 << s.bits;
-    hipLaunchKernelGGL(digit_count_kernel, dim3((unsigned)s.nblk), dim3(TE_THREADS), 0, st, rows, keys,
-                       p * s.bits, bins, s.nblk, counts);
-    hipLaunchKernelGGL(digit_scan_kernel, dim3((unsigned)tv_cdiv(bins, TE_THREADS / 64)), dim3(TE_THREADS), 0,
-                       st, bins, s.nblk, counts, totals);
-    hipLaunchKernelGGL(digit_scatter_kernel, dim3((unsigned)s.nblk), dim3(TE_THREADS), 0, st, rows, keys,
-                       p * s.bits, s.bits, s.nblk, counts, totals, to);
-    TV_LAUNCH_CHECK("tv_scaled_embedding_bwd");
-    keys.pairs = to;
-  }
+  launch_sort(s, rows, Keys{ids, nullptr, num_tokens, padding_id}, ws, st);
+  TV_LAUNCH_CHECK("tv_scaled_embedding_bwd");
+  const uint2 *sorted = (const uint2 *)(ws + s.pairs0);
   float *part = (float *)(ws + s.part);
-#define TE_GO(D, W) launch_sums<D, W>(s, rows, dim, num_tokens, pairs[0], dout, dout_stride, scale, dweight, part, st)
+#define TE_GO(D, W) launch_sums<D, W>(s, rows, dim, num_tokens, sorted, dout, dout_stride, scale, dweight, part, st)
   if (weight_dtype == TV_DTYPE_F32 && out_dtype == TV_DTYPE_F32) TE_GO(float, float);
   else if (weight_dtype == TV_DTYPE_F32 && out_dtype == TV_DTYPE_BF16) TE_GO(__bf16, float);
   else if (weight_dtype == TV_DTYPE_F32) TE_GO(_Float16, float);

@@ -1,0 +1,267 @@
+// Host side of operators whose cost in Python would be several times that of their kernels: an
+// autograd node for the scaled embedding (a node written in Python needs the interpreter's lock in
+// autograd's own thread: 30 us of a 90 us forward + backward) and the addresses of many tensors at
+// once (150 parameters: 60 us as Python loops, 3 here).  The kernels are reached through the C-ABI, by
+// the addresses that `bind` is given, so that both sides use the same build of the library.
+#include <Python.h>
+
+#include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
+#include <c10/core/DeviceGuard.h>
+#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <string>
+
+#include "../../include/tracevae_hip.h"
+
+namespace {
+
+struct {
+  decltype(&tv_last_error) last_error;
+  decltype(&tv_scaled_embedding_fwd) fwd;
+  decltype(&tv_scaled_embedding_bwd) bwd;
+  decltype(&tv_scaled_embedding_bwd_workspace_bytes) bwd_bytes;
+} lib;
+PyObject *library_error, *memory_error;           // hip.HipLibraryError, torch.OutOfMemoryError
+
+struct LibraryError : std::runtime_error {
+  using std::runtime_error::runtime_error;
+};
+
+void check(int rc, const char *name) {
+  if (rc != TV_OK) throw LibraryError(std::string(name) + " failed (" + std::to_string(rc) + "): " + lib.last_error());
+}
+
+int dtype_code(at::ScalarType t) {
+  switch (t) {
+    case at::kFloat: return TV_DTYPE_F32;
+    case at::kBFloat16: return TV_DTYPE_BF16;
+    case at::kHalf: return TV_DTYPE_F16;
+    default: return -1;
+  }
+}
+at::ScalarType dtype_of(int64_t code) {
+  return code == TV_DTYPE_F32 ? at::kFloat : code == TV_DTYPE_BF16 ? at::kBFloat16 : at::kHalf;
+}
+
+void *stream_of(const at::Tensor &t) {
+  return (void *)c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream();
+}
+
+// what tracevae_amd.ops.scaled_embedding has checked: a [tokens, dim] table with contiguous rows,
+// contiguous int64 ids on its device, types that go together
+class ScaledEmbedding : public torch::autograd::Function<ScaledEmbedding> {
+ public:
+  static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &weight,
+                            const at::Tensor &ids, double scale, int64_t padding_id, int64_t out_code) {
+    const c10::DeviceGuard guard(weight.device());
+    const int64_t tokens = weight.size(0), dim = weight.size(1), rows = ids.numel();
+    auto shape = ids.sizes().vec();
+    shape.push_back(dim);
+    at::Tensor out = at::empty(shape, weight.options().dtype(dtype_of(out_code)).requires_grad(false));
+    check(lib.fwd(rows, dim, tokens, dtype_code(weight.scalar_type()), (int)out_code, weight.const_data_ptr(),
+                  tokens > 1 ? weight.stride(0) : dim, ids.const_data_ptr<int64_t>(), padding_id, (float)scale,
+                  out.mutable_data_ptr(), dim, stream_of(weight)),
+          "tv_scaled_embedding_fwd");
+    ctx->save_for_backward({ids});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["sizes"] = std::vector<int64_t>{tokens, dim, (int64_t)dtype_code(weight.scalar_type()),
+                                                    out_code, padding_id};
+    return out;
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx,
+                                                 torch::autograd::variable_list grads) {
+    const at::Tensor ids = ctx->get_saved_variables()[0];
+    const double scale = ctx->saved_data["scale"].toDouble();
+    const auto sizes = ctx->saved_data["sizes"].toIntVector();
+    const int64_t tokens = sizes[0], dim = sizes[1], rows = ids.numel();
+    const c10::DeviceGuard guard(ids.device());
+    at::Tensor dw;
+    {
+      const at::AutoGradMode no_grad(false);
+      at::Tensor dout = grads[0].reshape({rows, dim});
+      const bool rows_apart = rows <= 1 || dout.stride(0) >= dim, dense_rows = dim <= 1 || dout.stride(1) == 1;
+      if (!rows_apart || !dense_rows) dout = dout.contiguous();
+      dw = at::empty({tokens, dim}, dout.options().dtype(dtype_of(sizes[2])));
+      // (a buffer of this call: a captured graph has it to itself)
+      const int64_t bytes = lib.bwd_bytes(rows, dim, tokens);
+      at::Tensor ws = at::empty({bytes}, dout.options().dtype(at::kByte));
+      check(lib.bwd(rows, dim, tokens, (int)sizes[2], (int)sizes[3], ids.const_data_ptr<int64_t>(), sizes[4],
+                    (float)scale, dout.const_data_ptr(), rows > 1 ? dout.stride(0) : dim, dw.mutable_data_ptr(),
+                    ws.mutable_data_ptr(), bytes, stream_of(ids)),
+            "tv_scaled_embedding_bwd");
+    }
+    if (at::GradMode::is_enabled() && grads[0].requires_grad()) {
+      // no second derivative: differentiating the result again is an error, as in the other operators
+      auto error = std::make_shared<torch::autograd::DelayedError>(
+          "trying to differentiate scaled_embedding twice: its gradient is once differentiable", 1);
+      dw.set_requires_grad(true);
+      dw = (*error)({dw})[0];
+    }
+    return {dw, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+// ---------------------------------------------------------------------------------------
+bool address_of(PyObject *o, void **to) {
+  *to = PyLong_AsVoidPtr(o);
+  return *to != nullptr || !PyErr_Occurred();
+}
+
+PyObject *bind(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  void *a[4];
+  if (n != 6) {
+    PyErr_SetString(PyExc_TypeError, "bind takes four addresses and two exception classes");
+    return nullptr;
+  }
+  for (int i = 0; i < 4; ++i)
+    if (!address_of(args[i], &a[i])) return nullptr;
+  lib.last_error = (decltype(lib.last_error))a[0];
+  lib.fwd = (decltype(lib.fwd))a[1];
+  lib.bwd = (decltype(lib.bwd))a[2];
+  lib.bwd_bytes = (decltype(lib.bwd_bytes))a[3];
+  Py_INCREF(args[4]);
+  Py_INCREF(args[5]);
+  library_error = args[4];
+  memory_error = args[5];
+  Py_RETURN_NONE;
+}
+
+template <typename F> PyObject *guarded(F f) {
+  try {
+    return f();
+  } catch (const LibraryError &e) {
+    PyErr_SetString(library_error, e.what());
+  } catch (const python_error &) {
+    // (set already)
+  } catch (const c10::OutOfMemoryError &e) {
+    PyErr_SetString(memory_error, e.what());
+  } catch (const std::exception &e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+  }
+  return nullptr;
+}
+
+PyObject *scaled_embedding(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  if (n != 5 || !THPVariable_Check(args[0]) || !THPVariable_Check(args[1])) {
+    PyErr_SetString(PyExc_TypeError, "scaled_embedding(weight, ids, scale, padding_id, out_dtype)");
+    return nullptr;
+  }
+  const double scale = PyFloat_AsDouble(args[2]);
+  const int64_t padding = PyLong_AsLongLong(args[3]), out_code = PyLong_AsLongLong(args[4]);
+  if (PyErr_Occurred()) return nullptr;
+  return guarded([&]() -> PyObject * {
+    const at::Tensor &weight = THPVariable_Unpack(args[0]), &ids = THPVariable_Unpack(args[1]);
+    at::Tensor out;
+    {
+      struct Released {                           // (also when an exception passes)
+        PyThreadState *state = PyEval_SaveThread();
+        ~Released() { PyEval_RestoreThread(state); }
+      } released;
+      out = ScaledEmbedding::apply(weight, ids, scale, padding, out_code);
+    }
+    return THPVariable_Wrap(out);
+  });
+}
+
+// adamw_addresses(params, grads or None, dtypes, sizes, planned, param_out, grad_out): the addresses
+// of the parameters and of their gradients (0: none) into two int64 arrays; dtypes (int), sizes and
+// planned (int64) are arrays of the optimizer.  Returns (moved, kept): whether an address is not the
+// planned one, and the contiguous copies of strided gradients, which have to live until the launch.
+PyObject *adamw_addresses(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  if (n != 7 || !PyList_Check(args[0]) || !(args[1] == Py_None || PyList_Check(args[1]))) {
+    PyErr_SetString(PyExc_TypeError, "adamw_addresses(params, grads, dtypes, sizes, planned, param_out, grad_out)");
+    return nullptr;
+  }
+  void *a[5];
+  for (int i = 0; i < 5; ++i)
+    if (!address_of(args[2 + i], &a[i])) return nullptr;
+  const int *dtypes = (const int *)a[0];
+  const int64_t *sizes = (const int64_t *)a[1], *planned = (const int64_t *)a[2];
+  int64_t *param_out = (int64_t *)a[3], *grad_out = (int64_t *)a[4];
+  const Py_ssize_t count = PyList_GET_SIZE(args[0]);
+  if (args[1] != Py_None && PyList_GET_SIZE(args[1]) != count) {
+    PyErr_Format(PyExc_ValueError, "%zd gradients for %zd parameters", PyList_GET_SIZE(args[1]), count);
+    return nullptr;
+  }
+  return guarded([&]() -> PyObject * {
+    PyObject *kept = nullptr;
+    bool moved = false;
+    auto refuse = [&](const std::string &text) -> PyObject * {
+      Py_XDECREF(kept);
+      PyErr_SetString(PyExc_TypeError, text.c_str());
+      return nullptr;
+    };
+    for (Py_ssize_t i = 0; i < count; ++i) {
+      PyObject *po = PyList_GET_ITEM(args[0], i), *go = args[1] == Py_None ? nullptr : PyList_GET_ITEM(args[1], i);
+      if (!THPVariable_Check(po) || (go && go != Py_None && !THPVariable_Check(go)))
+        return refuse("parameters and gradients are tensors");
+      const at::Tensor &p = THPVariable_Unpack(po);
+      if (p.numel() != sizes[i] || dtype_code(p.scalar_type()) != dtypes[i] || !p.is_contiguous())
+        return refuse("parameter " + std::to_string(i) + " is not of the size, type or layout that the optimizer was made for");
+      param_out[i] = (int64_t)p.const_data_ptr();
+      moved |= param_out[i] != planned[i];
+      at::Tensor g;
+      if (args[1] == Py_None) g = p.grad();
+      else if (go != Py_None) g = THPVariable_Unpack(go);
+      if (!g.defined()) {
+        grad_out[i] = 0;
+        continue;
+      }
+      if (g.layout() != at::kStrided || g.scalar_type() != p.scalar_type() || g.device() != p.device() ||
+          g.sizes() != p.sizes())
+        return refuse("gradient " + std::to_string(i) + " must be a dense tensor of the parameter's type (" +
+                      c10::toString(p.scalar_type()) + "), shape and device, got " + c10::toString(g.scalar_type()) +
+                      " on " + g.device().str());
+      if (!g.is_contiguous()) {
+        g = g.detach().contiguous();
+        if (!kept) kept = PyList_New(0);
+        PyObject *o = kept ? THPVariable_Wrap(g) : nullptr;
+        if (!o || PyList_Append(kept, o) != 0) {
+          Py_XDECREF(o);
+          Py_XDECREF(kept);
+          return nullptr;
+        }
+        Py_DECREF(o);
+      }
+      grad_out[i] = (int64_t)g.const_data_ptr();
+    }
+    if (!kept) {
+      Py_INCREF(Py_None);
+      kept = Py_None;
+    }
+    return Py_BuildValue("(NN)", PyBool_FromLong(moved), kept);
+  });
+}
+
+// the parameters have been written to by a kernel
+PyObject *written(PyObject *, PyObject *params) {
+  if (!PyList_Check(params)) {
+    PyErr_SetString(PyExc_TypeError, "written(params)");
+    return nullptr;
+  }
+  return guarded([&]() -> PyObject * {
+    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(params); ++i) {
+      if (!THPVariable_Check(PyList_GET_ITEM(params, i))) continue;
+      const at::Tensor &p = THPVariable_Unpack(PyList_GET_ITEM(params, i));
+      if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
+    }
+    Py_RETURN_NONE;
+  });
+}
+
+PyMethodDef methods[] = {
+    {"bind", (PyCFunction)(void (*)(void))bind, METH_FASTCALL, nullptr},
+    {"scaled_embedding", (PyCFunction)(void (*)(void))scaled_embedding, METH_FASTCALL, nullptr},
+    {"adamw_addresses", (PyCFunction)(void (*)(void))adamw_addresses, METH_FASTCALL, nullptr},
+    {"written", written, METH_O, nullptr},
+    {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__torch_host(void) { return PyModule_Create(&module); }

@@ -5,12 +5,13 @@ module raises.  Tensors are passed as raw device pointers (`tensor.data_ptr()`),
 stream is torch's current HIP stream.
 """
 import ctypes
+import importlib.util
 import os
 from typing import Dict, Optional, Tuple
 
 import torch
 
-__all__ = ['lib', 'call', 'query', 'array_type', 'ptr', 'stream', 'library_path', 'header_path', 'SIGNATURES',
+__all__ = ['lib', 'host', 'call', 'query', 'array_type', 'ptr', 'stream', 'library_path', 'header_path', 'SIGNATURES',
            'HipLibraryError']
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -85,6 +86,27 @@ def lib() -> ctypes.CDLL:
             fn.restype = _CTYPES[ret]
         _lib = handle
     return _lib
+
+
+_host = None
+
+
+def host():
+    """The extension module `csrc/_torch_host.so` (built with the library): operators whose cost in
+    Python would be several times that of their kernels.  It calls the C-ABI of `lib()`."""
+    global _host
+    if _host is None:
+        path = os.path.join(_HERE, 'csrc', '_torch_host.so')
+        if not os.path.isfile(path):
+            raise HipLibraryError(f'{path} is missing: build it with `make -C tracevae_amd/csrc`')
+        spec = importlib.util.spec_from_file_location('_torch_host', path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.bind(*(ctypes.cast(getattr(lib(), name), ctypes.c_void_p).value for name in (
+            'tv_last_error', 'tv_scaled_embedding_fwd', 'tv_scaled_embedding_bwd',
+            'tv_scaled_embedding_bwd_workspace_bytes')), HipLibraryError, torch.OutOfMemoryError)
+        _host = module
+    return _host
 
 
 def ptr(t) -> Optional[int]:

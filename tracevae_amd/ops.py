@@ -1222,39 +1222,6 @@ def embedding(weight, ids, extra_cols: int = 0):
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # TV_DTYPE_*
 
 
-class _ScaledEmbedding(Function):
-    @staticmethod
-    def forward(ctx, weight, ids, scale: float, padding_id: int, out_dtype):
-        rows, (v, dim) = ids.numel(), weight.shape
-        out = torch.empty([rows, dim], dtype=out_dtype, device=weight.device)
-        hip.call('tv_scaled_embedding_fwd', rows, dim, v, _DTYPES[weight.dtype], _DTYPES[out_dtype],
-                 weight.data_ptr(), weight.stride(0) if v > 1 else dim, ids.data_ptr(), padding_id,
-                 scale, out.data_ptr(), dim)
-        ctx.save_for_backward(ids)
-        ctx.args = (v, dim, weight.dtype, out_dtype, scale, padding_id)
-        return out.view(ids.shape + (dim,))
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout):
-        (ids,) = ctx.saved_tensors
-        v, dim, dtype, out_dtype, scale, padding_id = ctx.args
-        rows = ids.numel()
-        dout = dout.reshape(rows, dim)
-        if rows > 1 and (dout.stride(0) < dim or (dim > 1 and dout.stride(1) != 1)):
-            dout = dout.contiguous()
-        elif rows == 1 and dim > 1 and dout.stride(1) != 1:
-            dout = dout.contiguous()
-        dw = torch.empty([v, dim], dtype=dtype, device=dout.device)
-        # (not the shared scratch of `_workspace`: a captured graph has this buffer to itself)
-        nbytes = hip.query('tv_scaled_embedding_bwd_workspace_bytes', rows, dim, v)
-        ws = torch.empty([nbytes], dtype=torch.uint8, device=dout.device)
-        hip.call('tv_scaled_embedding_bwd', rows, dim, v, _DTYPES[dtype], _DTYPES[out_dtype],
-                 ids.data_ptr(), padding_id, scale, dout.data_ptr(),
-                 dout.stride(0) if rows > 1 else dim, dw.data_ptr(), ws.data_ptr(), nbytes)
-        return dw, None, None, None, None
-
-
 def scaled_embedding(weight, ids, scale: float = 1.0, padding_idx: Optional[int] = None,
                      out_dtype: Optional[torch.dtype] = None):
     """`scale * weight[ids]`, rounded once to `out_dtype` (default: the table's type; a 16-bit type
@@ -1265,21 +1232,22 @@ def scaled_embedding(weight, ids, scale: float = 1.0, padding_idx: Optional[int]
     if not weight.is_cuda or ids.device != weight.device:
         raise hip.HipLibraryError(f'weight is on {weight.device}, ids on {ids.device}: the accelerated '
                                   f'path runs on the GPU only (there is no CPU fallback)')
-    if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
-        raise ValueError(f'weight must be [tokens, dim], got {tuple(weight.shape)}')
+    dtype = weight.dtype
+    if out_dtype is None:
+        out_dtype = dtype
+    if dtype not in _DTYPES or out_dtype not in _DTYPES \
+            or (out_dtype != dtype and dtype != torch.float32):
+        raise TypeError(f'a table of {dtype} does not give rows of {out_dtype}')
     if ids.dtype != torch.int64:
         raise TypeError(f'ids must be torch.int64, got {ids.dtype}')
-    out_dtype = weight.dtype if out_dtype is None else out_dtype
-    if weight.dtype not in _DTYPES or out_dtype not in _DTYPES \
-            or (out_dtype != weight.dtype and weight.dtype != torch.float32):
-        raise TypeError(f'a table of {weight.dtype} does not give rows of {out_dtype}')
-    if weight.stride(1) != 1 or weight.stride(0) < weight.shape[1]:
-        weight = weight.contiguous()
-    padding_id = -1 if padding_idx is None else int(padding_idx)
-    if weight.device.index != torch._C._cuda_getDevice():
-        with torch.cuda.device(weight.device):
-            return _ScaledEmbedding.apply(weight, ids.contiguous(), float(scale), padding_id, out_dtype)
-    return _ScaledEmbedding.apply(weight, ids.contiguous(), float(scale), padding_id, out_dtype)
+    if not weight.is_contiguous():
+        if weight.dim() == 2 and (weight.stride(1) != 1 or weight.stride(0) < weight.shape[1]):
+            weight = weight.contiguous()
+    if weight.dim() != 2 or weight.numel() == 0:
+        raise ValueError(f'weight must be [tokens, dim], got {tuple(weight.shape)}')
+    return hip.host().scaled_embedding(weight, ids if ids.is_contiguous() else ids.contiguous(),
+                                       scale, -1 if padding_idx is None else padding_idx,
+                                       _DTYPES[out_dtype])
 
 
 class _LatDecInput(Function):

@@ -71,7 +71,10 @@ class AdamW(object):
         self._sizes = hip.array_type(ctypes.c_int64, n)(*[p.numel() for p in self.params])
         self._dtypes = hip.array_type(ctypes.c_int, n)(*[_DTYPES[p.dtype] for p in self.params])
         self._decay = hip.array_type(ctypes.c_double, n)(*decay)
-        self._kinds = [(p.dtype, p.shape) for p in self.params]
+        # addresses of one step: parameters, gradients
+        self._addresses = hip.array_type(ctypes.c_int64, 2 * n)()
+        self._at_params = ctypes.addressof(self._addresses)
+        self._at_grads = self._at_params + 8 * n
         lib = hip.lib()
         total = int(lib.tv_adamw_state_elements(n, self._sizes))
         self.offsets, at = [], 0
@@ -116,11 +119,11 @@ class AdamW(object):
 
     def _make_plan(self) -> None:
         n = len(self.params)
-        where = [p.data_ptr() for p in self.params]
+        where = hip.array_type(ctypes.c_int64, n)(*[p.data_ptr() for p in self.params])
         nbytes = int(hip.lib().tv_adamw_plan_bytes(n, self._sizes))
         image = torch.zeros((nbytes + 7) // 8, dtype=torch.int64)
         self._call_host('tv_adamw_plan', n, self._sizes, self._dtypes,
-                        hip.array_type(ctypes.c_void_p, n)(*where), self._decay,
+                        ctypes.addressof(where), self._decay,
                         image.data_ptr(), nbytes)
         self._plan_host, self._plan, self._where = image, image.to(self.device), where
 
@@ -166,26 +169,11 @@ class AdamW(object):
         if self.device.index != torch._C._cuda_getDevice():
             with torch.cuda.device(self.device):
                 return self.step(grads, global_clip_norm, guard, guard_kind, guard_host)
-        params = self.params
-        if grads is None:
-            grads = [p.grad for p in params]
-        elif len(grads) != len(params):
-            raise ValueError(f'{len(grads)} gradients for {len(params)} parameters')
-        where, held = [], []
-        for i, g in enumerate(grads):
-            if g is None:
-                where.append(None)
-                continue
-            if (g.dtype, g.shape) != self._kinds[i] or g.device != self.device \
-                    or g.layout != torch.strided:
-                raise TypeError(f'gradient {i} must be {self._kinds[i][0]} of '
-                                f'{tuple(self._kinds[i][1])} on {self.device}, got {g.dtype} of '
-                                f'{tuple(g.shape)} on {g.device} ({g.layout})')
-            if not g.is_contiguous():
-                g = g.contiguous()
-                held.append(g)
-            where.append(g.data_ptr())
-        if [p.data_ptr() for p in params] != self._where:
+        moved, kept = hip.host().adamw_addresses(
+            self.params, grads if grads is None or type(grads) is list else list(grads),
+            ctypes.addressof(self._dtypes), ctypes.addressof(self._sizes),
+            ctypes.addressof(self._where), self._at_params, self._at_grads)
+        if moved:
             if torch.cuda.is_current_stream_capturing():
                 raise hip.HipLibraryError('a parameter has moved since the last step: take one '
                                           'eager step before capturing')
@@ -197,11 +185,12 @@ class AdamW(object):
             moments = (s['exp_avg8'].data_ptr(), s['exp_rms8'].data_ptr(),
                        s['exp_avg_scale'].data_ptr(), s['exp_rms_scale'].data_ptr())
         hip.call('tv_adamw_step', self._plan_host.data_ptr(), self._plan.data_ptr(),
-                 hip.array_type(ctypes.c_void_p, len(params))(*where), self.state_bits, *moments,
+                 self._at_grads, self.state_bits, *moments,
                  s['master'].data_ptr() if 'master' in s else None, self._control.data_ptr(), clip,
                  self.grad_norm.data_ptr() if clip else None, self.seed, hip.ptr(guard),
                  guard_kind if guard is not None else 0,
                  guard_host.data_ptr() if guard_host is not None else None,
                  self._workspace.data_ptr(), self._workspace.numel() * 8)
-        torch.autograd.graph.increment_version(params)
+        del kept                                   # (queued: the stream keeps the memory in order)
+        hip.host().written(self.params)
         return self.grad_norm if clip else None
