@@ -23,8 +23,9 @@ def test_state_and_plan_sizes():
     lib = hip.lib()
     sizes = (I64 * 5)(1, 256, 257, 0, 4097)
     assert lib.tv_adamw_state_elements(5, sizes) == 256 + 256 + 512 + 0 + 4352
-    # one chunk of 4096 elements per started 4096
-    assert lib.tv_adamw_plan_bytes(5, sizes) - lib.tv_adamw_plan_bytes(4, sizes) == 40 + 2 * 8
+    # one entry per started 4096 elements, and one per tensor
+    grow = [lib.tv_adamw_plan_bytes(1, (I64 * 1)(n)) for n in (0, 1, 4096, 4097, 8193)]
+    assert grow[1] == grow[2] and grow[1] - grow[0] == grow[3] - grow[2] == grow[4] - grow[3] > 0
     assert lib.tv_adamw_state_elements(1, (I64 * 1)(-1)) == -1
     assert lib.tv_adamw_state_elements(2, (I64 * 2)(2 ** 60, 2 ** 60)) == -1
     assert lib.tv_adamw_plan_bytes(1, (I64 * 1)(-1)) == -1

@@ -30,30 +30,34 @@ template <int N, typename T> struct Some {
   typedef T V __attribute__((ext_vector_type(N)));
   typedef V Any __attribute__((aligned(sizeof(T))));
 };
-template <int N, typename T> __device__ __forceinline__ void load_n(const T *p, float (&x)[N]) {
+template <int N, typename T, bool PAST = false> __device__ __forceinline__ void load_n(const T *p, float (&x)[N]) {
   constexpr int M = N * sizeof(T) > 16 ? 16 / sizeof(T) : N;
   if constexpr (N == 1) {
     x[0] = (float)p[0];
   } else {
 #pragma unroll
     for (int k = 0; k < N; k += M) {
-      const typename Some<M, T>::V f = *reinterpret_cast<const typename Some<M, T>::Any *>(p + k);
+      typedef typename Some<M, T>::Any Any;
+      const Any *q = reinterpret_cast<const Any *>(p + k);
+      const typename Some<M, T>::V f = PAST ? __builtin_nontemporal_load(q) : *q;
 #pragma unroll
       for (int j = 0; j < M; ++j) x[k + j] = (float)f[j];
     }
   }
 }
-template <int N, typename T> __device__ __forceinline__ void store_n(T *p, const float (&x)[N]) {
+template <int N, typename T, bool PAST = false> __device__ __forceinline__ void store_n(T *p, const float (&x)[N]) {
   constexpr int M = N * sizeof(T) > 16 ? 16 / sizeof(T) : N;
   if constexpr (N == 1) {
     p[0] = (T)x[0];
   } else {
 #pragma unroll
     for (int k = 0; k < N; k += M) {
-      typename Some<M, T>::Any f;
+      typedef typename Some<M, T>::Any Any;
+      typename Some<M, T>::V f;
 #pragma unroll
       for (int j = 0; j < M; ++j) f[j] = (T)x[k + j];
-      *reinterpret_cast<typename Some<M, T>::Any *>(p + k) = f;
+      if (PAST) __builtin_nontemporal_store(f, reinterpret_cast<Any *>(p + k));
+      else *reinterpret_cast<Any *>(p + k) = f;
     }
   }
 }
@@ -69,7 +73,7 @@ __device__ __forceinline__ int64_t part_column(int64_t part, int n, int64_t dim)
 // ---------------------------------------------------------------------------------------
 // forward: 2^lg threads per row, ROWS rows per thread with their loads in flight together
 // ---------------------------------------------------------------------------------------
-template <typename W, typename O, int N, int ROWS>
+template <typename W, typename O, int N, int ROWS, bool PAST>
 __global__ __launch_bounds__(TE_THREADS) void lookup_kernel(int64_t rows, int64_t dim, int64_t vocab,
                                                             int parts, int lg, const W *__restrict__ weight,
                                                             int64_t weight_stride,
@@ -105,7 +109,7 @@ __global__ __launch_bounds__(TE_THREADS) void lookup_kernel(int64_t rows, int64_
 #pragma unroll
         for (int j = 0; j < N; ++j) x[k][j] *= scale;
       }
-      store_n<N, O>(out + r * out_stride + col, x[k]);
+      store_n<N, O, PAST>(out + r * out_stride + col, x[k]);
     }
   }
 }
@@ -369,8 +373,8 @@ __global__ __launch_bounds__(TE_THREADS) void tile_sums_kernel(
 #pragma unroll
     for (int k = 0; k < TE_BATCH; ++k) p[k] = next[k];
 #pragma unroll
-    for (int k = 0; k < TE_BATCH; ++k)            // (rows of padding are inside dout as well)
-      load_n<N, D>(dout + (int64_t)p[k].y * dout_stride + col, x[k]);
+    for (int k = 0; k < TE_BATCH; ++k)            // (rows of padding are inside dout as well; read once)
+      load_n<N, D, true>(dout + (int64_t)p[k].y * dout_stride + col, x[k]);
 #pragma unroll
     for (int k = 0; k < TE_BATCH; ++k) {          // the next pairs, on their way behind these rows
       const int64_t q = i + TE_BATCH + k;
@@ -550,14 +554,15 @@ void launch_lookup_n(int64_t rows, int64_t dim, int64_t vocab, const void *weigh
   int lg = 0;
   while ((1 << lg) < parts && lg < 8) ++lg;
   const int64_t per = TE_THREADS >> lg;
-  if (tv_cdiv(rows, per) >= 4096)
-    hipLaunchKernelGGL((lookup_kernel<W, O, N, 4>), dim3((unsigned)tv_cdiv(rows, per * 4)), dim3(TE_THREADS), 0,
-                       stream, rows, dim, vocab, parts, lg, (const W *)weight, weight_stride, ids, padding, scale,
-                       (O *)out, out_stride);
-  else
-    hipLaunchKernelGGL((lookup_kernel<W, O, N, 1>), dim3((unsigned)tv_cdiv(rows, per)), dim3(TE_THREADS), 0,
-                       stream, rows, dim, vocab, parts, lg, (const W *)weight, weight_stride, ids, padding, scale,
-                       (O *)out, out_stride);
+  // Four rows per thread where that leaves four workgroups per CU.  Rows of 128 MiB and more are written
+  // with the hint that they do not stay in the cache: lookup and one pass over its result take 177 us
+  // with it and 181 without at 256 MiB, 90 and 90 at 128, 42 and 41 at 64.
+  const bool four = tv_cdiv(rows, per) >= 4096, past = rows * dim * (int64_t)sizeof(O) >= ((int64_t)128 << 20);
+  auto kernel = !four ? lookup_kernel<W, O, N, 1, false>
+                      : past ? lookup_kernel<W, O, N, 4, true> : lookup_kernel<W, O, N, 4, false>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)tv_cdiv(rows, per * (four ? 4 : 1))), dim3(TE_THREADS), 0, stream, rows,
+                     dim, vocab, parts, lg, (const W *)weight, weight_stride, ids, padding, scale, (O *)out,
+                     out_stride);
 }
 template <typename W, typename O>
 void launch_lookup(int64_t rows, int64_t dim, int64_t vocab, const void *weight, int64_t weight_stride,

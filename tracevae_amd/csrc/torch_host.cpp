@@ -1,7 +1,7 @@
 // Host side of operators whose cost in Python would be several times that of their kernels: an
 // autograd node for the scaled embedding (a node written in Python needs the interpreter's lock in
 // autograd's own thread: 30 us of a 90 us forward + backward) and the addresses of many tensors at
-// once (150 parameters: 60 us as Python loops, 3 here).  The kernels are reached through the C-ABI, by
+// once (150 parameters: 60 us as Python loops, 5 here).  The kernels are reached through the C-ABI, by
 // the addresses that `bind` is given, so that both sides use the same build of the library.
 #include <Python.h>
 
@@ -14,6 +14,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <string>
+#include <vector>
 
 #include "../../include/tracevae_hip.h"
 
@@ -24,10 +25,14 @@ struct {
   decltype(&tv_scaled_embedding_fwd) fwd;
   decltype(&tv_scaled_embedding_bwd) bwd;
   decltype(&tv_scaled_embedding_bwd_workspace_bytes) bwd_bytes;
+  decltype(&tv_adamw_step) adamw_step;
 } lib;
 PyObject *library_error, *memory_error;           // hip.HipLibraryError, torch.OutOfMemoryError
 
-struct LibraryError : std::runtime_error {
+struct LibraryError : std::runtime_error {        // becomes hip.HipLibraryError
+  using std::runtime_error::runtime_error;
+};
+struct Mismatch : std::runtime_error {            // becomes TypeError
   using std::runtime_error::runtime_error;
 };
 
@@ -53,19 +58,25 @@ void *stream_of(const at::Tensor &t) {
 
 // what tracevae_amd.ops.scaled_embedding has checked: a [tokens, dim] table with contiguous rows,
 // contiguous int64 ids on its device, types that go together
+at::Tensor lookup(const at::Tensor &weight, const at::Tensor &ids, double scale, int64_t padding_id, int64_t out_code) {
+  const c10::DeviceGuard guard(weight.device());
+  const int64_t tokens = weight.size(0), dim = weight.size(1), rows = ids.numel();
+  at::DimVector shape(ids.sizes());
+  shape.push_back(dim);
+  at::Tensor out = at::empty(shape, weight.options().dtype(dtype_of(out_code)).requires_grad(false));
+  check(lib.fwd(rows, dim, tokens, dtype_code(weight.scalar_type()), (int)out_code, weight.const_data_ptr(),
+                tokens > 1 ? weight.stride(0) : dim, ids.const_data_ptr<int64_t>(), padding_id, (float)scale,
+                out.mutable_data_ptr(), dim, stream_of(weight)),
+        "tv_scaled_embedding_fwd");
+  return out;
+}
+
 class ScaledEmbedding : public torch::autograd::Function<ScaledEmbedding> {
  public:
   static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &weight,
                             const at::Tensor &ids, double scale, int64_t padding_id, int64_t out_code) {
-    const c10::DeviceGuard guard(weight.device());
-    const int64_t tokens = weight.size(0), dim = weight.size(1), rows = ids.numel();
-    auto shape = ids.sizes().vec();
-    shape.push_back(dim);
-    at::Tensor out = at::empty(shape, weight.options().dtype(dtype_of(out_code)).requires_grad(false));
-    check(lib.fwd(rows, dim, tokens, dtype_code(weight.scalar_type()), (int)out_code, weight.const_data_ptr(),
-                  tokens > 1 ? weight.stride(0) : dim, ids.const_data_ptr<int64_t>(), padding_id, (float)scale,
-                  out.mutable_data_ptr(), dim, stream_of(weight)),
-          "tv_scaled_embedding_fwd");
+    const int64_t tokens = weight.size(0), dim = weight.size(1);
+    const at::Tensor out = lookup(weight, ids, scale, padding_id, out_code);
     ctx->save_for_backward({ids});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["sizes"] = std::vector<int64_t>{tokens, dim, (int64_t)dtype_code(weight.scalar_type()),
@@ -113,21 +124,22 @@ bool address_of(PyObject *o, void **to) {
 }
 
 PyObject *bind(PyObject *, PyObject *const *args, Py_ssize_t n) {
-  void *a[4];
-  if (n != 6) {
-    PyErr_SetString(PyExc_TypeError, "bind takes four addresses and two exception classes");
+  void *a[5];
+  if (n != 7) {
+    PyErr_SetString(PyExc_TypeError, "bind takes five addresses and two exception classes");
     return nullptr;
   }
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < 5; ++i)
     if (!address_of(args[i], &a[i])) return nullptr;
   lib.last_error = (decltype(lib.last_error))a[0];
   lib.fwd = (decltype(lib.fwd))a[1];
   lib.bwd = (decltype(lib.bwd))a[2];
   lib.bwd_bytes = (decltype(lib.bwd_bytes))a[3];
-  Py_INCREF(args[4]);
+  lib.adamw_step = (decltype(lib.adamw_step))a[4];
   Py_INCREF(args[5]);
-  library_error = args[4];
-  memory_error = args[5];
+  Py_INCREF(args[6]);
+  library_error = args[5];
+  memory_error = args[6];
   Py_RETURN_NONE;
 }
 
@@ -136,6 +148,8 @@ template <typename F> PyObject *guarded(F f) {
     return f();
   } catch (const LibraryError &e) {
     PyErr_SetString(library_error, e.what());
+  } catch (const Mismatch &e) {
+    PyErr_SetString(PyExc_TypeError, e.what());
   } catch (const python_error &) {
     // (set already)
   } catch (const c10::OutOfMemoryError &e) {
@@ -162,103 +176,89 @@ PyObject *scaled_embedding(PyObject *, PyObject *const *args, Py_ssize_t n) {
         PyThreadState *state = PyEval_SaveThread();
         ~Released() { PyEval_RestoreThread(state); }
       } released;
-      out = ScaledEmbedding::apply(weight, ids, scale, padding, out_code);
+      out = at::GradMode::is_enabled() && weight.requires_grad()
+                ? ScaledEmbedding::apply(weight, ids, scale, padding, out_code)
+                : lookup(weight, ids, scale, padding, out_code);
     }
     return THPVariable_Wrap(out);
   });
 }
 
-// adamw_addresses(params, grads or None, dtypes, sizes, planned, param_out, grad_out): the addresses
-// of the parameters and of their gradients (0: none) into two int64 arrays; dtypes (int), sizes and
-// planned (int64) are arrays of the optimizer.  Returns (moved, kept): whether an address is not the
-// planned one, and the contiguous copies of strided gradients, which have to live until the launch.
-PyObject *adamw_addresses(PyObject *, PyObject *const *args, Py_ssize_t n) {
-  if (n != 7 || !PyList_Check(args[0]) || !(args[1] == Py_None || PyList_Check(args[1]))) {
-    PyErr_SetString(PyExc_TypeError, "adamw_addresses(params, grads, dtypes, sizes, planned, param_out, grad_out)");
+// adamw_step(params, grads or None, dtypes, sizes, planned, addresses, plan_host, plan_device, bits,
+// moment1, moment2, scale1, scale2, master, control, clip, norm, seed, guard, guard_kind, guard_host,
+// workspace, workspace_bytes, stream): tv_adamw_step with the gradients' addresses.  dtypes (int), sizes
+// and planned (int64: the parameters' addresses in the plan) are arrays of the optimizer, addresses is
+// its int64 scratch.  False: a parameter is not where the plan has it, nothing was done.
+PyObject *adamw_step(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  if (n != 24 || !PyList_Check(args[0]) || !(args[1] == Py_None || PyList_Check(args[1]))) {
+    PyErr_SetString(PyExc_TypeError, "adamw_step takes a list of parameters, a list of gradients or None, and 22 more");
     return nullptr;
   }
-  void *a[5];
-  for (int i = 0; i < 5; ++i)
-    if (!address_of(args[2 + i], &a[i])) return nullptr;
-  const int *dtypes = (const int *)a[0];
-  const int64_t *sizes = (const int64_t *)a[1], *planned = (const int64_t *)a[2];
-  int64_t *param_out = (int64_t *)a[3], *grad_out = (int64_t *)a[4];
-  const Py_ssize_t count = PyList_GET_SIZE(args[0]);
-  if (args[1] != Py_None && PyList_GET_SIZE(args[1]) != count) {
-    PyErr_Format(PyExc_ValueError, "%zd gradients for %zd parameters", PyList_GET_SIZE(args[1]), count);
+  void *a[24] = {};
+  double clip = 0.0;
+  for (int i = 2; i < 24; ++i) {
+    if (i == 15) clip = PyFloat_AsDouble(args[i]);
+    else if (i == 17) a[i] = (void *)(intptr_t)PyLong_AsUnsignedLongLongMask(args[i]);     // the seed
+    else if (args[i] != Py_None) a[i] = PyLong_AsVoidPtr(args[i]);
+    if (PyErr_Occurred()) return nullptr;
+  }
+  const int *dtypes = (const int *)a[2];
+  const int64_t *sizes = (const int64_t *)a[3], *planned = (const int64_t *)a[4];
+  const void **grad_at = (const void **)a[5];
+  PyObject *params = args[0], *grads = args[1] == Py_None ? nullptr : args[1];
+  const Py_ssize_t count = PyList_GET_SIZE(params);
+  if (grads && PyList_GET_SIZE(grads) != count) {
+    PyErr_Format(PyExc_ValueError, "%zd gradients for %zd parameters", PyList_GET_SIZE(grads), count);
     return nullptr;
   }
   return guarded([&]() -> PyObject * {
-    PyObject *kept = nullptr;
+    std::vector<at::Tensor> kept;                 // contiguous copies, until the launch
     bool moved = false;
-    auto refuse = [&](const std::string &text) -> PyObject * {
-      Py_XDECREF(kept);
-      PyErr_SetString(PyExc_TypeError, text.c_str());
-      return nullptr;
-    };
     for (Py_ssize_t i = 0; i < count; ++i) {
-      PyObject *po = PyList_GET_ITEM(args[0], i), *go = args[1] == Py_None ? nullptr : PyList_GET_ITEM(args[1], i);
-      if (!THPVariable_Check(po) || (go && go != Py_None && !THPVariable_Check(go)))
-        return refuse("parameters and gradients are tensors");
+      PyObject *po = PyList_GET_ITEM(params, i), *go = grads ? PyList_GET_ITEM(grads, i) : Py_None;
+      if (!THPVariable_Check(po) || (go != Py_None && !THPVariable_Check(go)))
+        throw Mismatch("parameters and gradients are tensors");
       const at::Tensor &p = THPVariable_Unpack(po);
       if (p.numel() != sizes[i] || dtype_code(p.scalar_type()) != dtypes[i] || !p.is_contiguous())
-        return refuse("parameter " + std::to_string(i) + " is not of the size, type or layout that the optimizer was made for");
-      param_out[i] = (int64_t)p.const_data_ptr();
-      moved |= param_out[i] != planned[i];
+        throw Mismatch("parameter " + std::to_string(i) +
+                       " no longer has the size, type or layout that the optimizer was made for");
+      moved |= (int64_t)p.const_data_ptr() != planned[i];
       at::Tensor g;
-      if (args[1] == Py_None) g = p.grad();
+      if (!grads) g = p.grad();
       else if (go != Py_None) g = THPVariable_Unpack(go);
       if (!g.defined()) {
-        grad_out[i] = 0;
+        grad_at[i] = nullptr;
         continue;
       }
       if (g.layout() != at::kStrided || g.scalar_type() != p.scalar_type() || g.device() != p.device() ||
           g.sizes() != p.sizes())
-        return refuse("gradient " + std::to_string(i) + " must be a dense tensor of the parameter's type (" +
-                      c10::toString(p.scalar_type()) + "), shape and device, got " + c10::toString(g.scalar_type()) +
-                      " on " + g.device().str());
+        throw Mismatch("gradient " + std::to_string(i) + " must be a dense tensor of the parameter's type (" +
+                       c10::toString(p.scalar_type()) + "), shape and device, got " +
+                       c10::toString(g.scalar_type()) + " on " + g.device().str());
       if (!g.is_contiguous()) {
         g = g.detach().contiguous();
-        if (!kept) kept = PyList_New(0);
-        PyObject *o = kept ? THPVariable_Wrap(g) : nullptr;
-        if (!o || PyList_Append(kept, o) != 0) {
-          Py_XDECREF(o);
-          Py_XDECREF(kept);
-          return nullptr;
-        }
-        Py_DECREF(o);
+        kept.push_back(g);
       }
-      grad_out[i] = (int64_t)g.const_data_ptr();
+      grad_at[i] = g.const_data_ptr();
     }
-    if (!kept) {
-      Py_INCREF(Py_None);
-      kept = Py_None;
-    }
-    return Py_BuildValue("(NN)", PyBool_FromLong(moved), kept);
-  });
-}
-
-// the parameters have been written to by a kernel
-PyObject *written(PyObject *, PyObject *params) {
-  if (!PyList_Check(params)) {
-    PyErr_SetString(PyExc_TypeError, "written(params)");
-    return nullptr;
-  }
-  return guarded([&]() -> PyObject * {
-    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(params); ++i) {
-      if (!THPVariable_Check(PyList_GET_ITEM(params, i))) continue;
+    if (moved) Py_RETURN_FALSE;
+    check(lib.adamw_step(a[6], a[7], grad_at, (int)(intptr_t)a[8], a[9], a[10], (float *)a[11], (float *)a[12],
+                         (float *)a[13], a[14], clip, (double *)a[16], (int64_t)(intptr_t)a[17],
+                         (const float *)a[18], (int)(intptr_t)a[19], (float *)a[20], a[21],
+                         (int64_t)(intptr_t)a[22], a[23]),
+          "tv_adamw_step");
+    for (Py_ssize_t i = 0; i < count; ++i) {      // written by a kernel
       const at::Tensor &p = THPVariable_Unpack(PyList_GET_ITEM(params, i));
       if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
     }
-    Py_RETURN_NONE;
+    Py_RETURN_TRUE;
   });
 }
 
 PyMethodDef methods[] = {
     {"bind", (PyCFunction)(void (*)(void))bind, METH_FASTCALL, nullptr},
     {"scaled_embedding", (PyCFunction)(void (*)(void))scaled_embedding, METH_FASTCALL, nullptr},
-    {"adamw_addresses", (PyCFunction)(void (*)(void))adamw_addresses, METH_FASTCALL, nullptr},
-    {"written", written, METH_O, nullptr},
+    {"adamw_step", (PyCFunction)(void (*)(void))adamw_step, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -104,7 +104,7 @@ def host():
         spec.loader.exec_module(module)
         module.bind(*(ctypes.cast(getattr(lib(), name), ctypes.c_void_p).value for name in (
             'tv_last_error', 'tv_scaled_embedding_fwd', 'tv_scaled_embedding_bwd',
-            'tv_scaled_embedding_bwd_workspace_bytes')), HipLibraryError, torch.OutOfMemoryError)
+            'tv_scaled_embedding_bwd_workspace_bytes', 'tv_adamw_step')), HipLibraryError, torch.OutOfMemoryError)
         _host = module
     return _host
 

@@ -20,7 +20,7 @@ BLOCK = 256                                                            # TV_ADAM
 
 class AdamW(object):
     """One AdamW step over all of `params` per `step()`: three launches with clipping, two without
-    (per 384 tensors).
+    (one or two more for every 384 tensors).
 
         m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2
         p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
@@ -71,10 +71,7 @@ class AdamW(object):
         self._sizes = hip.array_type(ctypes.c_int64, n)(*[p.numel() for p in self.params])
         self._dtypes = hip.array_type(ctypes.c_int, n)(*[_DTYPES[p.dtype] for p in self.params])
         self._decay = hip.array_type(ctypes.c_double, n)(*decay)
-        # addresses of one step: parameters, gradients
-        self._addresses = hip.array_type(ctypes.c_int64, 2 * n)()
-        self._at_params = ctypes.addressof(self._addresses)
-        self._at_grads = self._at_params + 8 * n
+        self._addresses = hip.array_type(ctypes.c_int64, n)()
         lib = hip.lib()
         total = int(lib.tv_adamw_state_elements(n, self._sizes))
         self.offsets, at = [], 0
@@ -102,7 +99,6 @@ class AdamW(object):
         self._write_control(0)
         self._workspace = zeros(int(lib.tv_adamw_workspace_bytes(n)) // 8, torch.float64)
         self.grad_norm = torch.zeros((), dtype=torch.float64, device=self.device)
-        self._plan_host, self._plan, self._where = None, None, None
         self._make_plan()
 
     # -- set-up ------------------------------------------------------------------------
@@ -126,6 +122,9 @@ class AdamW(object):
                         ctypes.addressof(where), self._decay,
                         image.data_ptr(), nbytes)
         self._plan_host, self._plan, self._where = image, image.to(self.device), where
+        self._arrays = tuple(ctypes.addressof(x) for x in (self._dtypes, self._sizes, self._where,
+                                                           self._addresses))
+        self._plan_at = (self._plan_host.data_ptr(), self._plan.data_ptr())
 
     # -- hyper-parameters and state ----------------------------------------------------
     def set_lr(self, lr: float) -> None:
@@ -169,28 +168,24 @@ class AdamW(object):
         if self.device.index != torch._C._cuda_getDevice():
             with torch.cuda.device(self.device):
                 return self.step(grads, global_clip_norm, guard, guard_kind, guard_host)
-        moved, kept = hip.host().adamw_addresses(
-            self.params, grads if grads is None or type(grads) is list else list(grads),
-            ctypes.addressof(self._dtypes), ctypes.addressof(self._sizes),
-            ctypes.addressof(self._where), self._at_params, self._at_grads)
-        if moved:
-            if torch.cuda.is_current_stream_capturing():
-                raise hip.HipLibraryError('a parameter has moved since the last step: take one '
-                                          'eager step before capturing')
-            self._make_plan()
         s, clip = self.state, float(global_clip_norm or 0.0)
         if self.state_bits == 32:
             moments = (s['exp_avg'].data_ptr(), s['exp_avg_sq'].data_ptr(), None, None)
         else:
             moments = (s['exp_avg8'].data_ptr(), s['exp_rms8'].data_ptr(),
                        s['exp_avg_scale'].data_ptr(), s['exp_rms_scale'].data_ptr())
-        hip.call('tv_adamw_step', self._plan_host.data_ptr(), self._plan.data_ptr(),
-                 self._at_grads, self.state_bits, *moments,
-                 s['master'].data_ptr() if 'master' in s else None, self._control.data_ptr(), clip,
-                 self.grad_norm.data_ptr() if clip else None, self.seed, hip.ptr(guard),
-                 guard_kind if guard is not None else 0,
-                 guard_host.data_ptr() if guard_host is not None else None,
-                 self._workspace.data_ptr(), self._workspace.numel() * 8)
-        del kept                                   # (queued: the stream keeps the memory in order)
-        hip.host().written(self.params)
+        if grads is not None and type(grads) is not list:
+            grads = list(grads)
+        step = hip.host().adamw_step
+        while not step(self.params, grads, *self._arrays, *self._plan_at, self.state_bits, *moments,
+                       s['master'].data_ptr() if 'master' in s else None, self._control.data_ptr(),
+                       clip, self.grad_norm.data_ptr() if clip else None, self.seed, hip.ptr(guard),
+                       guard_kind if guard is not None else 0,
+                       guard_host.data_ptr() if guard_host is not None else None,
+                       self._workspace.data_ptr(), self._workspace.numel() * 8, hip.stream()):
+            # a parameter is not where it was
+            if torch.cuda.is_current_stream_capturing():
+                raise hip.HipLibraryError('a parameter has moved since the last step: take one '
+                                          'eager step before capturing')
+            self._make_plan()
         return self.grad_norm if clip else None
