@@ -502,7 +502,8 @@ int tv_embedding_bwd(int64_t rows, int64_t dim, int64_t num_operations, const in
  * weight / out types (TV_DTYPE_*): equal, or an fp32 table with 16-bit rows; dout has out's type,
  * dweight weight's, [num_tokens, dim] dense.  Row strides in elements; no alignment beyond the
  * type's is needed (rows at multiples of 16 bytes are the fastest).  Sums are fp32 in a fixed
- * order, rounded once.  rows, num_tokens < 2^31 - 1; dim <= 65536.
+ * order, rounded once.  num_tokens <= 2^29, dim <= 65536, and rows * L < 2^33, where L is dim / 4
+ * rounded up to 16, 32 or a multiple of 64 (2^29 rows of up to 64 columns, 2^25 of 1024).
  * Workspace of the backward pass: 16-byte aligned, tv_scaled_embedding_bwd_workspace_bytes. */
 int tv_scaled_embedding_fwd(int64_t rows, int64_t dim, int64_t num_tokens, int weight_dtype,
                             int out_dtype, const void *weight, int64_t weight_stride,
@@ -751,7 +752,7 @@ int tv_optim_step_guarded(int kind, int64_t n, float *param, const float *grad, 
  *   tv_optim_step_guarded: a step that is skipped changes nothing, the step counter included.
  *   norm_out (nullable, device): ||g||, with clip_norm > 0 only.  workspace:
  *   tv_adamw_workspace_bytes(count) bytes, used with clip_norm > 0 only.  Calls on one state
- *   must be ordered (one stream, or events).
+ *   must be ordered (one stream, or events); gradients do not overlap parameters or state.
  * ---------------------------------------------------------------------------------- */
 int64_t tv_adamw_state_elements(int64_t count, const int64_t *sizes);
 int64_t tv_adamw_plan_bytes(int64_t count, const int64_t *sizes);

@@ -43,7 +43,8 @@ def test_plan_refuses():
                        (([100, 50], [4096, None]), b'null'),
                        (([100], [4096], [3]), b'dtype'),
                        (([100], [4096], [0], [-0.5]), b'decay'),
-                       (([100], [4096], [0], [float('nan')]), b'decay')):
+                       (([100], [4096], [0], [float('nan')]), b'decay'),
+                       (([100], [4096], [0], [float('inf')]), b'decay')):
         assert _plan(*args)[0] == -1
         assert text in lib.tv_last_error(), text
     assert _plan([100, 0], [4096, None])[0] == 0                   # an empty tensor has no address
@@ -59,7 +60,8 @@ def test_control_refuses():
     assert int(image[0]) == 3 and f[1:7].tolist() == [1e-3, 0.5, 0.25, 1e-8, 0.125, 0.015625]
     for bad in ((-1, 1e-3, 0.9, 0.99, 1e-8), (0, -1e-3, 0.9, 0.99, 1e-8), (0, 1e-3, 1.0, 0.99, 1e-8),
                 (0, 1e-3, 0.9, 1.0, 1e-8), (0, 1e-3, -0.1, 0.9, 1e-8), (0, 1e-3, 0.9, 0.99, -1.0),
-                (0, float('nan'), 0.9, 0.99, 1e-8)):
+                (0, float('nan'), 0.9, 0.99, 1e-8), (0, float('inf'), 0.9, 0.99, 1e-8),
+                (0, 1e-3, 0.9, 0.99, float('inf')), (0, 1e-3, float('nan'), 0.99, 1e-8)):
         assert lib.tv_adamw_control(*bad, image.data_ptr()) == -1, bad
     assert lib.tv_adamw_control(0, 1e-3, 0.9, 0.99, 1e-8, None) == -1
 

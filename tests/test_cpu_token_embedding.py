@@ -15,7 +15,8 @@ def test_refusals_before_any_launch():
     for kw in (dict(rows=-1), dict(dim=0), dict(v=0), dict(wt=3), dict(ot=-1), dict(wt=1, ot=0), dict(wt=1, ot=2),
                dict(wt=2, ot=1), dict(ws=7), dict(os=7), dict(w=None), dict(ids=None), dict(out=None),
                dict(w=one + 2), dict(out=one + 1), dict(ids=one + 4), dict(rows=2 ** 31), dict(v=2 ** 31),
-               dict(dim=65537, ws=70000, os=70000), dict(wt=0, ot=1, out=one + 1)):
+               dict(dim=65537, ws=70000, os=70000), dict(v=2 ** 29 + 1), dict(rows=2 ** 29),
+               dict(rows=2 ** 25, dim=1025, ws=1025, os=1025), dict(wt=0, ot=1, out=one + 1)):
         assert fwd(**kw) == -1, kw
         assert b'tv_scaled_embedding_fwd' in lib.tv_last_error()
     assert fwd(rows=0, w=None, ids=None, out=None) == 0
@@ -31,7 +32,8 @@ def test_refusals_before_any_launch():
                      (dict(dw=one + 2), -1), (dict(dout=one + 2), -1), (dict(ws=one + 8), -1), (dict(n=need - 1), -3),
                      (dict(rows=2 ** 31), -1)):
         assert bwd(**kw) == code, kw
-    for bad in ((-1, 8, 10), (4, 0, 10), (4, 8, 0), (2 ** 31, 8, 10), (4, 65537, 10), (4, 8, 2 ** 31)):
+    for bad in ((-1, 8, 10), (4, 0, 10), (4, 8, 0), (2 ** 31, 8, 10), (4, 65537, 10), (4, 8, 2 ** 31),
+                (2 ** 29, 8, 10), (2 ** 25, 1025, 10), (4, 8, 2 ** 29 + 1)):
         assert lib.tv_scaled_embedding_bwd_workspace_bytes(*bad) == -1
     assert lib.tv_scaled_embedding_bwd_workspace_bytes(0, 8, 10) == 0
 

@@ -442,8 +442,31 @@ def test_refusals(device):
             opt.step([g])
     with pytest.raises(hip.HipLibraryError):
         opt.step([p.clone()], -1.0)
-    with pytest.raises(ValueError):
-        opt.set_lr(-1.0)
+    for lr in (-1.0, math.nan, math.inf):
+        with pytest.raises(ValueError):
+            opt.set_lr(lr)
+    for guard in (torch.zeros(1), torch.zeros(1, device=device, dtype=torch.float64), torch.zeros(2, device=device)):
+        with pytest.raises(TypeError):
+            opt.step([p.clone()], None, guard, 1)
+    for host in (torch.zeros(1, dtype=torch.float64, pin_memory=True), torch.zeros(1, device=device)):
+        with pytest.raises(TypeError):
+            opt.step([p.clone()], None, torch.zeros(1, device=device), 1, host)
+    opt.state['exp_avg'] = torch.zeros(1, device=device)              # (a copy of the dict)
+    assert opt.state['exp_avg'].numel() == 256
+    q = torch.zeros(10, device=device, requires_grad=True)
+    other = AdamW([q])
+    q.grad = torch.ones(10, device=device)
+    for data in (torch.zeros(10), torch.zeros(11, device=device)):
+        keep = q.data
+        q.grad = None
+        q.data = data
+        with pytest.raises(TypeError):
+            other.step()
+        q.data = keep
+    sparse = torch.zeros(10, device=device).to_sparse()
+    with pytest.raises(TypeError):
+        opt.step([sparse])
+    assert other.steps == 0
     with pytest.raises(hip.HipLibraryError):
         opt.step([p.clone()], 1.0, torch.zeros(1, device=device), 1, torch.zeros(1))   # not pinned
     assert opt.steps == 0

@@ -169,6 +169,25 @@ def test_difference_quotient_and_two_uses(device):
     assert torch.equal(w.grad, 2 * dw)
 
 
+def test_no_second_derivative_and_no_changed_ids(device):
+    from tracevae_amd import ops
+    w = torch.randn(50, 16, device=device, requires_grad=True)
+    ids = torch.randint(0, 50, (100,), device=device)
+    d = torch.randn(100, 16, device=device, requires_grad=True)
+    (dw,) = torch.autograd.grad(ops.scaled_embedding(w, ids, 2.0), w, d, create_graph=True)
+    want = torch.autograd.grad(ops.scaled_embedding(w, ids, 2.0), w, d.detach())[0]
+    assert torch.equal(dw.detach(), want)
+    with pytest.raises(RuntimeError, match='twice'):
+        dw.sum().backward()
+    out = ops.scaled_embedding(w, ids, 2.0)
+    ids.fill_(3)                                          # as with torch's own lookup
+    with pytest.raises(RuntimeError, match='modified'):
+        out.sum().backward()
+    with torch.no_grad():
+        assert not ops.scaled_embedding(w, ids, 2.0).requires_grad
+    assert not ops.scaled_embedding(w.detach(), ids, 2.0).requires_grad
+
+
 def test_more_than_2_to_the_31_elements(device):
     """bf16 rows of 2^21 + 5 tokens by 1030 columns: positions beyond 32 bits in the rows and in their
     gradient (4.3 GB each)."""

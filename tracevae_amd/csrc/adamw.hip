@@ -463,7 +463,8 @@ extern "C" int tv_adamw_control(int64_t step, double lr, double beta1, double be
   TV_REQUIRE(step >= 0, "tv_adamw_control: step counts from 0 (steps taken so far)");
   TV_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0,
              "tv_adamw_control: the betas lie in [0, 1)");
-  TV_REQUIRE(eps >= 0.0 && lr >= 0.0, "tv_adamw_control: lr and eps are not negative");
+  TV_REQUIRE(eps >= 0.0 && eps < INFINITY && lr >= 0.0 && lr < INFINITY,
+             "tv_adamw_control: lr and eps are finite and not negative");
   Control c = {};
   c.step = step;
   c.lr = lr;
@@ -515,8 +516,8 @@ extern "C" int tv_adamw_plan(int64_t count, const int64_t *sizes, const int *dty
                "tv_adamw_plan: tensor %lld has an unknown dtype %d", (long long)i, dtypes[i]);
     TV_REQUIRE((params[i] || sizes[i] == 0) && ((uintptr_t)params[i] & (uintptr_t)(width - 1)) == 0,
                "tv_adamw_plan: tensor %lld has a null or misaligned address", (long long)i);
-    TV_REQUIRE(weight_decay[i] >= 0.0, "tv_adamw_plan: the weight decay of tensor %lld is negative",
-               (long long)i);
+    TV_REQUIRE(weight_decay[i] >= 0.0 && weight_decay[i] < INFINITY,
+               "tv_adamw_plan: the weight decay of tensor %lld is negative or infinite", (long long)i);
     tensors[i] = Tensor{sizes[i], dtypes[i], (int32_t)chunk};
     for (int64_t k = 0; k < tv_cdiv(sizes[i], AW_CHUNK); ++k) {
       const int64_t left = sizes[i] - k * AW_CHUNK;

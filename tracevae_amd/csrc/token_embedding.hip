@@ -506,7 +506,6 @@ struct Shape {
   int nblk, passes, bits;
   int64_t pairs0, pairs1, counts, part, bytes;
 };
-constexpr int64_t TE_MAX_BLOCKS = ((int64_t)1 << 32) / TE_JOIN_THREADS - 1;     // 2^32 threads per launch
 inline int64_t align256(int64_t x) { return (x + 255) & ~(int64_t)255; }
 
 // lanes of one row: groups of 16, 32 or 64
@@ -542,8 +541,10 @@ inline Shape shape_of(int64_t rows, int64_t dim, int64_t vocab) {
 }
 
 inline bool sizes_ok(int64_t rows, int64_t dim, int64_t vocab) {
-  // (so that sorted positions and tokens fit 32 bits, and tiles * slabs a grid)
-  return rows >= 0 && rows < INT32_MAX && dim >= 1 && dim <= (1 << 16) && vocab >= 1 && vocab < INT32_MAX;
+  // (sorted positions and tokens fit 32 bits; a launch has less than 2^32 threads: 4 for each table row,
+  // and no more than one for every 4 elements of the rows)
+  return rows >= 0 && rows < INT32_MAX && dim >= 1 && dim <= (1 << 16) && vocab >= 1 && vocab <= (1 << 29) &&
+         rows * lanes_of(dim, 4) < ((int64_t)1 << 33);
 }
 
 template <typename W, typename O, int N>

@@ -186,17 +186,17 @@ PyObject *scaled_embedding(PyObject *, PyObject *const *args, Py_ssize_t n) {
 
 // adamw_step(params, grads or None, dtypes, sizes, planned, addresses, plan_host, plan_device, bits,
 // moment1, moment2, scale1, scale2, master, control, clip, norm, seed, guard, guard_kind, guard_host,
-// workspace, workspace_bytes, stream): tv_adamw_step with the gradients' addresses.  dtypes (int), sizes
+// workspace, workspace_bytes, stream, device): tv_adamw_step with the gradients' addresses.  dtypes (int), sizes
 // and planned (int64: the parameters' addresses in the plan) are arrays of the optimizer, addresses is
 // its int64 scratch.  False: a parameter is not where the plan has it, nothing was done.
 PyObject *adamw_step(PyObject *, PyObject *const *args, Py_ssize_t n) {
-  if (n != 24 || !PyList_Check(args[0]) || !(args[1] == Py_None || PyList_Check(args[1]))) {
-    PyErr_SetString(PyExc_TypeError, "adamw_step takes a list of parameters, a list of gradients or None, and 22 more");
+  if (n != 25 || !PyList_Check(args[0]) || !(args[1] == Py_None || PyList_Check(args[1]))) {
+    PyErr_SetString(PyExc_TypeError, "adamw_step takes a list of parameters, a list of gradients or None, and 23 more");
     return nullptr;
   }
-  void *a[24] = {};
+  void *a[25] = {};
   double clip = 0.0;
-  for (int i = 2; i < 24; ++i) {
+  for (int i = 2; i < 25; ++i) {
     if (i == 15) clip = PyFloat_AsDouble(args[i]);
     else if (i == 17) a[i] = (void *)(intptr_t)PyLong_AsUnsignedLongLongMask(args[i]);     // the seed
     else if (args[i] != Py_None) a[i] = PyLong_AsVoidPtr(args[i]);
@@ -207,6 +207,7 @@ PyObject *adamw_step(PyObject *, PyObject *const *args, Py_ssize_t n) {
   const void **grad_at = (const void **)a[5];
   PyObject *params = args[0], *grads = args[1] == Py_None ? nullptr : args[1];
   const Py_ssize_t count = PyList_GET_SIZE(params);
+  const at::Device device(at::kCUDA, (at::DeviceIndex)(intptr_t)a[24]);
   if (grads && PyList_GET_SIZE(grads) != count) {
     PyErr_Format(PyExc_ValueError, "%zd gradients for %zd parameters", PyList_GET_SIZE(grads), count);
     return nullptr;
@@ -219,9 +220,10 @@ PyObject *adamw_step(PyObject *, PyObject *const *args, Py_ssize_t n) {
       if (!THPVariable_Check(po) || (go != Py_None && !THPVariable_Check(go)))
         throw Mismatch("parameters and gradients are tensors");
       const at::Tensor &p = THPVariable_Unpack(po);
-      if (p.numel() != sizes[i] || dtype_code(p.scalar_type()) != dtypes[i] || !p.is_contiguous())
+      if (p.numel() != sizes[i] || dtype_code(p.scalar_type()) != dtypes[i] || p.device() != device ||
+          !p.is_contiguous())
         throw Mismatch("parameter " + std::to_string(i) +
-                       " no longer has the size, type or layout that the optimizer was made for");
+                       " no longer has the size, type, device or layout that the optimizer was made for");
       moved |= (int64_t)p.const_data_ptr() != planned[i];
       at::Tensor g;
       if (!grads) g = p.grad();

@@ -83,17 +83,17 @@ class AdamW(object):
         def zeros(count, dtype=torch.float32):
             return torch.zeros(count, dtype=dtype, device=self.device)
 
-        self.state: Dict[str, torch.Tensor] = {}
+        self._state: Dict[str, torch.Tensor] = {}
         if state_bits == 32:
-            self.state.update(exp_avg=zeros(total), exp_avg_sq=zeros(total))
+            self._state.update(exp_avg=zeros(total), exp_avg_sq=zeros(total))
         else:
             for name in ('exp_avg', 'exp_rms'):
-                self.state[name + '8'] = zeros(total, torch.uint8).view(torch.float8_e4m3fn)
-                self.state[name + '_scale'] = zeros(total // BLOCK)
+                self._state[name + '8'] = zeros(total, torch.uint8).view(torch.float8_e4m3fn)
+                self._state[name + '_scale'] = zeros(total // BLOCK)
         if any(p.dtype != torch.float32 for p in self.params):
-            self.state['master'] = zeros(total)
+            self._state['master'] = zeros(total)
             for at, p in zip(self.offsets, self.params):
-                self.state['master'][at:at + p.numel()].copy_(p.detach().reshape(-1))
+                self._state['master'][at:at + p.numel()].copy_(p.detach().reshape(-1))
         self._control = zeros(int(lib.tv_adamw_control_bytes()) // 8, torch.int64)
         self._lr = self._control.view(torch.float64)[1]
         self._write_control(0)
@@ -130,8 +130,8 @@ class AdamW(object):
     def set_lr(self, lr: float) -> None:
         """The learning rate of the steps queued behind this call (a store on the current stream)."""
         lr = float(lr)
-        if not lr >= 0.0:
-            raise ValueError(f'the learning rate must not be negative, got {lr}')
+        if not 0.0 <= lr < float('inf'):
+            raise ValueError(f'the learning rate must be finite and not negative, got {lr}')
         if lr != self.lr:
             self.lr = lr
             self._lr.fill_(lr)
@@ -141,18 +141,23 @@ class AdamW(object):
         """Steps taken (waits for the GPU: the counter is there, skipped steps do not count)."""
         return int(self._control[0].item())
 
+    @property
+    def state(self) -> Dict[str, torch.Tensor]:
+        """The buffers by name (the optimizer's own: writing into them changes its state)."""
+        return dict(self._state)
+
     def state_dict(self) -> Dict[str, object]:
-        return dict({k: v.clone() for k, v in self.state.items()}, step=self.steps)
+        return dict({k: v.clone() for k, v in self._state.items()}, step=self.steps)
 
     def load_state_dict(self, state: Dict[str, object]) -> None:
         """Copies the buffers of a `state_dict()` of the same parameters and `state_bits`."""
-        if set(state) != set(self.state) | {'step'}:
-            raise ValueError(f'the state has {sorted(state)}, expected {sorted(self.state)} and step')
-        for k, v in self.state.items():
+        if set(state) != set(self._state) | {'step'}:
+            raise ValueError(f'the state has {sorted(state)}, expected {sorted(self._state)} and step')
+        for k, v in self._state.items():
             if tuple(state[k].shape) != tuple(v.shape) or state[k].dtype != v.dtype:
                 raise ValueError(f'{k} must be {v.dtype} of {tuple(v.shape)}, got {state[k].dtype} '
                                  f'of {tuple(state[k].shape)}')
-        for k, v in self.state.items():
+        for k, v in self._state.items():
             v.view(torch.uint8).copy_(state[k].to(self.device).contiguous().view(torch.uint8))
         self._write_control(int(state['step']))
 
@@ -168,7 +173,13 @@ class AdamW(object):
         if self.device.index != torch._C._cuda_getDevice():
             with torch.cuda.device(self.device):
                 return self.step(grads, global_clip_norm, guard, guard_kind, guard_host)
-        s, clip = self.state, float(global_clip_norm or 0.0)
+        if guard is not None and (guard.dtype != torch.float32 or guard.device != self.device
+                                  or guard.numel() != 1):
+            raise TypeError(f'the guard must be one float32 on {self.device}')
+        if guard_host is not None and (guard_host.dtype != torch.float32 or guard_host.numel() != 1
+                                       or guard_host.is_cuda):
+            raise TypeError('guard_host must be one float32 in pinned host memory')
+        s, clip = self._state, float(global_clip_norm or 0.0)
         if self.state_bits == 32:
             moments = (s['exp_avg'].data_ptr(), s['exp_avg_sq'].data_ptr(), None, None)
         else:
@@ -182,7 +193,8 @@ class AdamW(object):
                        clip, self.grad_norm.data_ptr() if clip else None, self.seed, hip.ptr(guard),
                        guard_kind if guard is not None else 0,
                        guard_host.data_ptr() if guard_host is not None else None,
-                       self._workspace.data_ptr(), self._workspace.numel() * 8, hip.stream()):
+                       self._workspace.data_ptr(), self._workspace.numel() * 8, hip.stream(),
+                       self.device.index):
             # a parameter is not where it was
             if torch.cuda.is_current_stream_capturing():
                 raise hip.HipLibraryError('a parameter has moved since the last step: take one '
