@@ -24,6 +24,7 @@ constexpr int TE_MAX_BITS = 10;                   // of a digit
 constexpr int TE_MAX_BINS = 1 << TE_MAX_BITS;
 constexpr int TE_BATCH = 8;                       // rows whose loads are in flight together
 constexpr int TE_JOIN_THREADS = 1024;
+constexpr int TE_LONG = 16;                       // tiles of a token that one group joins alone
 
 // N consecutive elements at any alignment of the type, in one access of up to 16 bytes
 template <int N, typename T> struct Some {
@@ -71,9 +72,13 @@ __device__ __forceinline__ int64_t part_column(int64_t part, int n, int64_t dim)
 }
 
 // ---------------------------------------------------------------------------------------
-// forward: 2^lg threads per row, ROWS rows per thread with their loads in flight together
+// Forward: 2^lg threads per row, ROWS rows per thread with their loads in flight together.  The rows are
+// stored past the caches: a lookup of 64, 256 and 512 MiB takes 20, 77 and 153 us so and 21, 85 and 178
+// without the hint, a lookup and one pass that reads its result 42, 177 and 343 against 41, 181 and 355 -
+// and without it what follows pays for the dirty lines (lookup and gradient of 32768 x 1024: 101 us
+// against 113).
 // ---------------------------------------------------------------------------------------
-template <typename W, typename O, int N, int ROWS, bool PAST>
+template <typename W, typename O, int N, int ROWS>
 __global__ __launch_bounds__(TE_THREADS) void lookup_kernel(int64_t rows, int64_t dim, int64_t vocab,
                                                             int parts, int lg, const W *__restrict__ weight,
                                                             int64_t weight_stride,
@@ -109,7 +114,7 @@ __global__ __launch_bounds__(TE_THREADS) void lookup_kernel(int64_t rows, int64_
 #pragma unroll
         for (int j = 0; j < N; ++j) x[k][j] *= scale;
       }
-      store_n<N, O, PAST>(out + r * out_stride + col, x[k]);
+      store_n<N, O, true>(out + r * out_stride + col, x[k]);
     }
   }
 }
@@ -233,30 +238,47 @@ __global__ __launch_bounds__(TE_SORT_THREADS) void digit_count_kernel(int64_t n,
   if ((int)threadIdx.x < bins) counts[(int64_t)blockIdx.x * bins + threadIdx.x] = hist[threadIdx.x];
 }
 
+// KEEP: a wave's run has at most that many rounds of 64 pairs, which stay in registers
+template <int KEEP>
 __global__ __launch_bounds__(TE_SORT_THREADS) void digit_scatter_kernel(
     int64_t n, Keys keys, int shift, int bits, int64_t items, int nblk,
     const uint32_t *__restrict__ counts, uint2 *__restrict__ out) {
   __shared__ uint32_t seen[TE_SORT_WAVES][TE_MAX_BINS];
   __shared__ uint32_t wave_sum[TE_SORT_WAVES];
   const int bins = 1 << bits, lane = threadIdx.x & 63, w = threadIdx.x >> 6, b = threadIdx.x;
+  const int64_t run = items / TE_SORT_WAVES;
+  const int64_t i0 = (int64_t)blockIdx.x * items + w * run;
+  const int64_t i1 = i0 + run < n ? i0 + run : n;
+  uint2 kept[KEEP > 0 ? KEEP : 1];
+  if (KEEP > 0) {
+#pragma unroll
+    for (int k = 0; k < KEEP; ++k)
+      kept[k] = i0 + k * 64 + lane < i1 ? keys.at(i0 + k * 64 + lane) : make_uint2(0u, 0u);
+  }
   for (int k = lane; k < bins; k += 64) seen[w][k] = 0;
   // the digit's pairs in the workgroups before this one, and in all
   uint32_t before = 0, total = 0;
   if (b < bins) {
-#pragma unroll 16
-    for (int k = 0; k < nblk; ++k) {
-      const uint32_t c = counts[(int64_t)k * bins + b];
-      before += k < (int)blockIdx.x ? c : 0u;
-      total += c;
+    for (int k0 = 0; k0 < nblk; k0 += 16) {
+      uint32_t c[16];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) c[k] = k0 + k < nblk ? counts[(int64_t)(k0 + k) * bins + b] : 0u;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        before += k0 + k < (int)blockIdx.x ? c[k] : 0u;
+        total += c[k];
+      }
     }
   }
-  const int64_t run = items / TE_SORT_WAVES;
-  const int64_t i0 = (int64_t)blockIdx.x * items + w * run;
-  const int64_t i1 = i0 + run < n ? i0 + run : n;
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll 4
-  for (int64_t i = i0 + lane; i < i1; i += 64)
-    atomicAdd(&seen[w][(keys.at(i).x >> shift) & (bins - 1)], 1u);
+  auto digit = [&](uint2 item) { return (item.x >> shift) & (bins - 1); };
+  if (KEEP > 0) {
+#pragma unroll
+    for (int k = 0; k < KEEP; ++k)
+      if (i0 + k * 64 + lane < i1) atomicAdd(&seen[w][digit(kept[k])], 1u);
+  } else {
+    for (int64_t i = i0 + lane; i < i1; i += 64) atomicAdd(&seen[w][digit(keys.at(i))], 1u);
+  }
   __syncthreads();
   uint32_t at = sort_exclusive_sum(b < bins ? total : 0u, wave_sum) + before;
   if (b < bins) {
@@ -268,11 +290,8 @@ __global__ __launch_bounds__(TE_SORT_THREADS) void digit_scatter_kernel(
     }
   }
   __syncthreads();
-  for (int64_t j = i0; j < i1; j += 64) {
-    const int64_t i = j + lane;
-    const bool in = i < i1;
-    const uint2 item = in ? keys.at(i) : make_uint2(0u, 0u);
-    const uint32_t d = (item.x >> shift) & (bins - 1);
+  auto place = [&](uint2 item, bool in) {
+    const uint32_t d = digit(item);
     const uint64_t same = same_digit(d, in, bits);
     const uint32_t below = (uint32_t)__popcll(same & ((1ull << lane) - 1ull));
     // (LDS accesses of one wave stay in order; the fences keep the compiler from moving them)
@@ -281,6 +300,15 @@ __global__ __launch_bounds__(TE_SORT_THREADS) void digit_scatter_kernel(
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     if (in && below == 0) seen[w][d] += (uint32_t)__popcll(same);
     if (in) out[to] = item;
+  };
+  if (KEEP > 0) {
+#pragma unroll
+    for (int k = 0; k < KEEP; ++k) place(kept[k], i0 + k * 64 + lane < i1);
+  } else {
+    for (int64_t j = i0; j < i1; j += 64) {
+      const bool in = j + lane < i1;
+      place(in ? keys.at(j + lane) : make_uint2(0u, 0u), in);
+    }
   }
 }
 
@@ -396,7 +424,7 @@ __global__ __launch_bounds__(TE_THREADS) void tile_sums_kernel(
 }
 
 // The token that begins in tile t and goes on behind it: its slot there, then slot 0 of the tiles
-// that follow, in order.  A group of G lanes takes the tokens of one tile; a token of more than G
+// that follow, in order.  A group of G lanes takes the token of one tile; one of more than TE_LONG
 // tiles is left to the whole workgroup, whose groups take one run of its tiles each.
 template <typename W, int N, int G>
 __global__ __launch_bounds__(TE_JOIN_THREADS) void join_kernel(int64_t n, int64_t dim, int64_t vocab, int tile,
@@ -433,7 +461,6 @@ __global__ __launch_bounds__(TE_JOIN_THREADS) void join_kernel(int64_t n, int64_
   };
   int64_t t, col;
   const bool active = tile_of(group, t, col);
-  int64_t end = 0;
   if (lane == 0) long_end[group] = 0;
   const int64_t i0 = t * tile, i1 = i0 + tile;
   if (t < tiles && i1 < n) {
@@ -447,16 +474,16 @@ __global__ __launch_bounds__(TE_JOIN_THREADS) void join_kernel(int64_t n, int64_
       const uint64_t all = __ballot(in);
       const uint64_t mine = (G == 64 ? all : (all >> ((threadIdx.x & 63) & ~(G - 1)))) & (G == 64 ? ~0ull : ((1ull << (G & 63)) - 1ull));
       const int run = __popcll(mine);
-      if (run < G) {
-        end = t + 1 + run;
+      if (run < G && run <= TE_LONG) {
         float acc[N];
         load_n<N, float>(part + (t * 2 + 1) * dim + col, acc);
-        add(t + 1, end, col, acc);
+        add(t + 1, t + 1 + run, col, acc);
 #pragma unroll
         for (int j = 0; j < N; ++j) acc[j] *= scale;
         if (active) store_n<N, W>(dweight + (int64_t)cur * dim + col, acc);
       } else {
-        lo = t + 1 + G;
+        lo = t + 1 + run;
+        if (run < G) hi = lo;
         while (lo < hi) {
           const int64_t mid = (lo + hi) >> 1;
           if (sorted[mid * tile].x == cur) lo = mid + 1;
@@ -471,19 +498,23 @@ __global__ __launch_bounds__(TE_JOIN_THREADS) void join_kernel(int64_t n, int64_
     const int64_t to = long_end[g];
     if (to == 0) continue;
     const bool on = tile_of(g, t, col);
-    const int64_t count = to - (t + 1), each = (count + GROUPS - 1) / GROUPS;
+    const int64_t count = to - (t + 1);
+    const int64_t each = count > GROUPS * TE_BATCH ? (count + GROUPS - 1) / GROUPS : TE_BATCH;
+    const int used = (int)((count + each - 1) / each);
     const int64_t u0 = t + 1 + group * each < to ? t + 1 + group * each : to;
     const int64_t u1 = u0 + each < to ? u0 + each : to;
     float acc[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) acc[j] = 0.f;
     if (group == 0) load_n<N, float>(part + (t * 2 + 1) * dim + col, acc);
-    add(u0, u1, col, acc);
+    if (group < used) {
+      add(u0, u1, col, acc);
 #pragma unroll
-    for (int j = 0; j < N; ++j) sums[group][j * G + lane] = acc[j];
+      for (int j = 0; j < N; ++j) sums[group][j * G + lane] = acc[j];
+    }
     __syncthreads();
     if (group == 0) {
-      for (int k = 1; k < GROUPS; ++k)
+      for (int k = 1; k < used; ++k)
 #pragma unroll
         for (int j = 0; j < N; ++j) acc[j] += sums[k][j * G + lane];
 #pragma unroll
@@ -555,12 +586,9 @@ void launch_lookup_n(int64_t rows, int64_t dim, int64_t vocab, const void *weigh
   int lg = 0;
   while ((1 << lg) < parts && lg < 8) ++lg;
   const int64_t per = TE_THREADS >> lg;
-  // Four rows per thread where that leaves four workgroups per CU.  Rows of 128 MiB and more are written
-  // with the hint that they do not stay in the cache: lookup and one pass over its result take 177 us
-  // with it and 181 without at 256 MiB, 90 and 90 at 128, 42 and 41 at 64.
-  const bool four = tv_cdiv(rows, per) >= 4096, past = rows * dim * (int64_t)sizeof(O) >= ((int64_t)128 << 20);
-  auto kernel = !four ? lookup_kernel<W, O, N, 1, false>
-                      : past ? lookup_kernel<W, O, N, 4, true> : lookup_kernel<W, O, N, 4, false>;
+  // four rows per thread where that leaves four workgroups per CU
+  const bool four = tv_cdiv(rows, per) >= 4096;
+  auto kernel = four ? lookup_kernel<W, O, N, 4> : lookup_kernel<W, O, N, 1>;
   hipLaunchKernelGGL(kernel, dim3((unsigned)tv_cdiv(rows, per * (four ? 4 : 1))), dim3(TE_THREADS), 0, stream, rows,
                      dim, vocab, parts, lg, (const W *)weight, weight_stride, ids, padding, scale, (O *)out,
                      out_stride);
@@ -590,7 +618,9 @@ void launch_sort(const Shape &s, int64_t rows, Keys keys, char *ws, hipStream_t 
     uint2 *to = pairs[(s.passes - 1 - p) & 1];    // (the last pass writes pairs[0])
     hipLaunchKernelGGL(digit_count_kernel, dim3((unsigned)s.nblk), dim3(TE_SORT_THREADS), 0, stream, rows, keys,
                        p * s.bits, s.bits, s.items, counts);
-    hipLaunchKernelGGL(digit_scatter_kernel, dim3((unsigned)s.nblk), dim3(TE_SORT_THREADS), 0, stream, rows, keys,
+    auto scatter = s.items <= TE_SORT_THREADS ? digit_scatter_kernel<1>
+                   : s.items <= 4 * TE_SORT_THREADS ? digit_scatter_kernel<4> : digit_scatter_kernel<0>;
+    hipLaunchKernelGGL(scatter, dim3((unsigned)s.nblk), dim3(TE_SORT_THREADS), 0, stream, rows, keys,
                        p * s.bits, s.bits, s.items, s.nblk, counts, to);
     keys.pairs = to;
   }
