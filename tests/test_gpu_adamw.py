@@ -146,6 +146,17 @@ def test_steps_against_the_formula(device, bits, dtype, shift, clip):
 
 
 @pytest.mark.parametrize('bits', [32, 8])
+def test_eps_of_zero_leaves_the_padding_zero(device, bits):
+    from tracevae_amd.optim import AdamW
+    params = _params([(255,), (3, 5), (1,), (4097,)], torch.bfloat16, device, 31)
+    opt = AdamW(params, weight_decay=0.0, state_bits=bits, lr=1e-2, eps=0.0)
+    twin = Twin(opt, [0.0] * 4)
+    for k in range(2):
+        twin.step([torch.where(x.abs() < 1e-6, torch.full_like(x, 1e-3), x) for x in _grads(params, 32 + k)])
+    assert all(torch.isfinite(p).all() for p in params)
+
+
+@pytest.mark.parametrize('bits', [32, 8])
 def test_tensors_without_gradient_and_strided_gradients(device, bits):
     from tracevae_amd.optim import AdamW
     params = _params([(30, 40), (5,), (300,), (17, 2)], torch.float32, device, 2)

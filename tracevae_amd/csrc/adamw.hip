@@ -115,20 +115,26 @@ __device__ __forceinline__ void load4(const float *p, int i, float (&x)[4]) {
 __device__ __forceinline__ void store4(float *p, int i, const float (&x)[4]) {
   __builtin_nontemporal_store(F4{x[0], x[1], x[2], x[3]}, reinterpret_cast<F4 *>(p + i));
 }
+// the master: zeros behind n, whatever 0 / 0 the formula makes of the padding (eps = 0)
+__device__ __forceinline__ void store_master(float *p, int i, int n, const float (&x)[4]) {
+  float y[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) y[j] = i + j < n ? x[j] : 0.f;
+  store4(p, i, y);
+}
 
 // ---------------------------------------------------------------------------------------
 // ||g||: float64 squares, one partial per workgroup, summed in order by begin_kernel
 // ---------------------------------------------------------------------------------------
 template <typename T> __device__ __forceinline__ double chunk_sumsq(const T *g, int n) {
-  constexpr int ITS = AW_CHUNK / (4 * AW_THREADS);
   double acc = 0.0;
   if (n == AW_CHUNK) {                            // all loads of the chunk in flight at once
-    typename Four<T>::V x[ITS];                   // (without the hint: the step reads them again)
+    typename Four<T>::V x[AW_ITS];                  // (without the hint: the step reads them again)
 #pragma unroll
-    for (int it = 0; it < ITS; ++it)
+    for (int it = 0; it < AW_ITS; ++it)
       x[it] = *reinterpret_cast<const typename Four<T>::Any *>(g + it * 4 * AW_THREADS + (int)threadIdx.x * 4);
 #pragma unroll
-    for (int it = 0; it < ITS; ++it)
+    for (int it = 0; it < AW_ITS; ++it)
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc = fma((double)(float)x[it][j], (double)(float)x[it][j], acc);
   } else {
@@ -278,7 +284,7 @@ __device__ __forceinline__ void chunk_step32(T *p, const T *g, float *w, float *
     store4(p, i, n, px);
     store4(m, i, mx);
     store4(v, i, vx);
-    if (sizeof(T) != 4) store4(w, i, px);
+    if (sizeof(T) != 4) store_master(w, i, n, px);
   }
 }
 
@@ -394,7 +400,7 @@ __device__ __forceinline__ void chunk_step8(T *p, const T *g, float *w, uint32_t
       px[j] = moved8(sizeof(T) == 4 ? px[j] : master_of<T>(px[j], wx[j]), mf, rf, s);
     }
     store4(p, i, n, px);
-    if (sizeof(T) != 4) store4(w, i, px);
+    if (sizeof(T) != 4) store_master(w, i, n, px);
     __builtin_nontemporal_store(cm, m8 + i / 4);
     __builtin_nontemporal_store(cr, r8 + i / 4);
     if (lane == 0) {
