@@ -504,7 +504,8 @@ int tv_embedding_bwd(int64_t rows, int64_t dim, int64_t num_operations, const in
  * type's is needed (rows at multiples of 16 bytes are the fastest).  Sums are fp32 in a fixed
  * order, rounded once.  num_tokens <= 2^29, dim <= 65536, and rows * L < 2^33, where L is dim / 4
  * rounded up to 16, 32 or a multiple of 64 (2^29 rows of up to 64 columns, 2^25 of 1024).
- * Workspace of the backward pass: 16-byte aligned, tv_scaled_embedding_bwd_workspace_bytes. */
+ * Workspace of the backward pass: 16-byte aligned, tv_scaled_embedding_bwd_workspace_bytes (0 for up
+ * to 128 rows). */
 int tv_scaled_embedding_fwd(int64_t rows, int64_t dim, int64_t num_tokens, int weight_dtype,
                             int out_dtype, const void *weight, int64_t weight_stride,
                             const int64_t *ids, int64_t padding_id, float scale, void *out,
@@ -737,7 +738,8 @@ int tv_optim_step_guarded(int kind, int64_t n, float *param, const float *grad, 
  *     rounded up or down with the probabilities that keep the value on average, by a hash of
  *     (seed, step, element): same seed, same bits.  A positive sqrt(v) keeps a positive code; an
  *     infinite or NaN moment becomes the NaN code and leaves its neighbours alone; a block whose
- *     scale would be below 2^-126 is stored as zeros.
+ *     scale would be below 2^-126 is stored as zeros.  Everything up to codes and scales is float64,
+ *     m as two products and a sum, each rounded.
  *   master: fp32, needed if any parameter has 16 bits (otherwise NULL).
  *
  * tv_adamw_plan writes the table of tensors and chunks into HOST memory; the caller keeps it and a

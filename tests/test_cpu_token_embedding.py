@@ -21,10 +21,11 @@ def test_refusals_before_any_launch():
         assert b'tv_scaled_embedding_fwd' in lib.tv_last_error()
     assert fwd(rows=0, w=None, ids=None, out=None) == 0
 
-    need = lib.tv_scaled_embedding_bwd_workspace_bytes(4, 8, 10)
+    assert lib.tv_scaled_embedding_bwd_workspace_bytes(128, 8, 10) == 0
+    need = lib.tv_scaled_embedding_bwd_workspace_bytes(400, 8, 10)
     assert need > 0
 
-    def bwd(rows=4, dim=8, v=10, wt=0, ot=0, ids=one, dout=one, ds=8, dw=one, ws=one, n=need):
+    def bwd(rows=400, dim=8, v=10, wt=0, ot=0, ids=one, dout=one, ds=8, dw=one, ws=one, n=need):
         return lib.tv_scaled_embedding_bwd(rows, dim, v, wt, ot, ids, -1, 1.0, dout, ds, dw, ws, n, None)
 
     for kw, code in ((dict(rows=-1), -1), (dict(dim=0), -1), (dict(v=0), -1), (dict(wt=1, ot=0), -1), (dict(ids=None), -1),

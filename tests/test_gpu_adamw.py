@@ -146,6 +146,24 @@ def test_steps_against_the_formula(device, bits, dtype, shift, clip):
 
 
 @pytest.mark.parametrize('bits', [32, 8])
+def test_steps_with_and_without_clipping_in_turn(device, bits):
+    """A step without norm and guard over few tensors is one launch that counts by itself; others count in
+    a launch of their own: in turn, and with a tensor list too long for the first kind."""
+    from tracevae_amd.optim import AdamW
+    for shapes in (ODD, ODD + [(1024 * 4096 + 5,)]):
+        params = _params(shapes, torch.float32, device, 41)
+        opt = AdamW(params, weight_decay=0.01, state_bits=bits, **HYPER)
+        twin = Twin(opt, [0.01] * len(shapes))
+        guard = torch.zeros(1, device=device)
+        for k, clip in enumerate([None, 0.5, None, None, 2.0, None]):
+            twin.step(_grads(params, 42 + k), clip)
+            if k == 2:
+                opt.step([None] * len(shapes), None, guard, 1)
+                opt.step([None] * len(shapes))
+                twin.t += 2
+
+
+@pytest.mark.parametrize('bits', [32, 8])
 def test_eps_of_zero_leaves_the_padding_zero(device, bits):
     from tracevae_amd.optim import AdamW
     params = _params([(255,), (3, 5), (1,), (4097,)], torch.bfloat16, device, 31)
@@ -260,7 +278,8 @@ def test_guarded_step(device, bits, kind, value, skipped):
 
 
 @pytest.mark.parametrize('bits', [32, 8])
-def test_captured_step_counts_on(device, bits):
+@pytest.mark.parametrize('clip', [1.0, None])
+def test_captured_step_counts_on(device, bits, clip):
     """One captured step, replayed with eager work of its own between the replays and another
     learning rate for the last ones, against an eager twin: equal bits after every replay."""
     from tracevae_amd.optim import AdamW
@@ -269,12 +288,12 @@ def test_captured_step_counts_on(device, bits):
     opt = AdamW(params, state_bits=bits, **HYPER)
     eager = AdamW(twins, state_bits=bits, **HYPER)
     g = _grads(params, 15)
-    opt.step(g, 1.0)
-    eager.step(g, 1.0)
+    opt.step(g, clip)
+    eager.step(g, clip)
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
-        opt.step(g, 1.0)
+        opt.step(g, clip)
     assert opt.steps == 1                                 # capturing runs nothing
     for k in range(5):
         for x, y in zip(g, _grads(params, 20 + k)):
@@ -285,7 +304,7 @@ def test_captured_step_counts_on(device, bits):
         graph.replay()
         junk = torch.randn(1000, device=device).sum().item()
         assert math.isfinite(junk)
-        eager.step(g, 1.0)
+        eager.step(g, clip)
         assert opt.steps == eager.steps == k + 2
         for a, b in zip(params, twins):
             assert torch.equal(a, b)

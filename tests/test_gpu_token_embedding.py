@@ -74,7 +74,9 @@ def _check(weight, ids, scale, padding, out_dtype, dout, device):
 
 @pytest.mark.parametrize('rows,vocab,dim', [(1, 1, 1), (2, 5, 3), (31, 1000, 40), (33, 7, 64), (257, 1023, 250),
                                            (1021, 997, 251), (5000, 1024, 40), (4097, 1025, 8), (300, 70001, 130),
-                                           (20000, 1000, 16), (9000, 5, 1027), (2049, 300000, 33)])
+                                           (20000, 1000, 16), (9000, 5, 1027), (2049, 300000, 33),
+                                           (64, 50, 5), (65, 17, 600), (128, 300, 72), (129, 300, 72), (100, 90000, 9),
+                                           (8192, 300, 20), (8193, 300, 20)])
 @pytest.mark.parametrize('kind', ['zipf', 'same', 'wild', 'runs'])
 def test_rows_and_gradient(device, rows, vocab, dim, kind):
     for k, (table, out_dtype) in enumerate(TYPES):

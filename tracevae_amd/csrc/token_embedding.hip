@@ -11,6 +11,12 @@
 // tile for a slab of columns and writes every token that begins and ends inside it; the sums of a
 // token that crosses tile borders go to a workspace and are joined in tile order.  Sums are fp32, in
 // a fixed order, rounded once; no atomics on floats, so results repeat bit for bit.
+//
+// Measured (kernels alone): lookup of 65536 x 4096 bf16 117 us (835 MB read and written,
+// 7.1 TB/s).  Gradient of 262144 x 512 bf16 over 1000 tokens, half of the rows on three of
+// them: sort 5 + 13, tiles 49 (268 MB read, 5.5 TB/s), join 15 us.  Of 32768 x 1024 bf16 into 50001 fp32
+// rows: sort 17, tiles and zero rows 45 (268 MB, 5.9 TB/s), join 10.  Of 25600 x 40 fp32 over 1000: sort 3
+// + 7, tiles 5, join 13; of 1021 x 251 fp16: sort 6, tiles 5, join 5 - a chain of dependent loads each.
 #include "tv_common.h"
 
 namespace {
@@ -18,6 +24,7 @@ namespace {
 constexpr int TE_THREADS = 256;
 constexpr int TE_SORT_THREADS = 1024;             // of a sort workgroup
 constexpr int TE_SORT_WAVES = TE_SORT_THREADS / 64;
+constexpr int TE_TINY = 128;                      // rows whose gradient is one launch
 constexpr int TE_SMALL = 8192;                    // rows that one workgroup sorts alone
 constexpr int TE_SORT_BLOCKS = 64;                // sort workgroups of longer lists, at most
 constexpr int TE_MAX_BITS = 10;                   // of a digit
@@ -161,7 +168,8 @@ __device__ __forceinline__ uint32_t sort_exclusive_sum(uint32_t c, uint32_t *wav
   return before;
 }
 
-// Up to TE_SMALL rows: all passes in one workgroup, the pairs in LDS between them.  Wave w takes the
+// Up to TE_SMALL rows: all passes in one workgroup, the pairs in LDS between them (1021 rows: 6 us; the
+// launches of the longer form take 10 at least).  Wave w takes the
 // w-th run of 64 * ROUNDS pairs; equal digits among 64 are ranked by lane, and the wave's own counter
 // carries the rank from round to round.
 template <int ROUNDS>
@@ -315,7 +323,9 @@ __global__ __launch_bounds__(TE_SORT_THREADS) void digit_scatter_kernel(
 // ---------------------------------------------------------------------------------------
 // sums over the sorted list
 // ---------------------------------------------------------------------------------------
-// rows of dW that no token names, 16 per wave: a binary search in the sorted list for each
+// Rows of dW that no token names, 16 per wave: a binary search in the sorted list for each.  They are
+// stored past the caches (50001 x 1024 fp32, three quarters of it zeros: 102 us for lookup and gradient
+// against 110 without; the rows that hold sums lose by it, 118).
 template <typename W>
 __device__ __forceinline__ void zero_absent_rows(int64_t wave, int64_t n, int64_t dim, int64_t vocab,
                                                  const uint2 *__restrict__ sorted, W *__restrict__ dweight) {
@@ -343,7 +353,7 @@ __device__ __forceinline__ void zero_absent_rows(int64_t wave, int64_t n, int64_
         float zero[M];
 #pragma unroll
         for (int j = 0; j < M; ++j) zero[j] = 0.f;
-        store_n<M, W>(row + part_column(part, M, dim), zero);
+        store_n<M, W, true>(row + part_column(part, M, dim), zero);
       }
     } else if (lane < dim) {
       row[lane] = (W)0.f;
@@ -525,6 +535,69 @@ __global__ __launch_bounds__(TE_JOIN_THREADS) void join_kernel(int64_t n, int64_
   }
 }
 
+// Up to TE_TINY rows: no sort.  A wave takes 16 table rows and a slab of columns, finds the rows of each
+// token with a ballot over all ids and adds them in order, eight loads in flight; table rows without any
+// become zeros.
+template <typename D, typename W, int N>
+__global__ __launch_bounds__(TE_THREADS) void tiny_sums_kernel(int n, int64_t dim, int64_t vocab, int64_t padding,
+                                                               const int64_t *__restrict__ ids,
+                                                               const D *__restrict__ dout, int64_t dout_stride,
+                                                               float scale, W *__restrict__ dweight) {
+  constexpr int K = TE_TINY / 64;
+  const int lane = threadIdx.x & 63;
+  const int64_t v0 = ((int64_t)blockIdx.x * (TE_THREADS / 64) + (threadIdx.x >> 6)) * 16;
+  if (v0 >= vocab) return;
+  const int64_t column_part = (int64_t)blockIdx.y * 64 + lane;
+  const bool active = column_part * N < dim;
+  const int64_t col = active ? part_column(column_part, N, dim) : 0;
+  uint32_t rel[K];                                // token - v0; vocab and beyond: none
+  uint64_t any = 0;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int i = k * 64 + lane;
+    const uint32_t token = i < n ? token_of(ids[i], vocab, padding) : (uint32_t)vocab;
+    rel[k] = token < (uint32_t)vocab ? token - (uint32_t)v0 : 0xffffffffu;
+    any |= __ballot(rel[k] < 16u);
+  }
+  for (int j = 0; j < 16 && v0 + j < vocab; ++j) {
+    float acc[N];
+#pragma unroll
+    for (int c = 0; c < N; ++c) acc[c] = 0.f;
+    bool named = false;
+    if (any) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        uint64_t rows = __ballot(rel[k] == (uint32_t)j);
+        named |= rows != 0;
+        while (rows) {
+          float x[TE_BATCH][N];
+          int count = 0;
+#pragma unroll
+          for (int b = 0; b < TE_BATCH; ++b) {
+            if (rows) {
+              const int r = k * 64 + __builtin_ctzll(rows);
+              rows &= rows - 1;
+              load_n<N, D, true>(dout + (int64_t)r * dout_stride + col, x[b]);
+              count = b + 1;
+            }
+          }
+#pragma unroll
+          for (int b = 0; b < TE_BATCH; ++b) {
+            if (b >= count) break;
+#pragma unroll
+            for (int c = 0; c < N; ++c) acc[c] += x[b][c];
+          }
+        }
+      }
+    }
+    if (named) {                                  // (0 * scale is no zero for an infinite scale)
+#pragma unroll
+      for (int c = 0; c < N; ++c) acc[c] *= scale;
+    }
+    if (active) store_n<N, W, true>(dweight + (v0 + j) * dim + col, acc);
+  }
+}
+
 template <typename W>
 __global__ __launch_bounds__(TE_THREADS) void zero_table_kernel(int64_t n, W *__restrict__ dweight) {
   const int64_t stride = (int64_t)gridDim.x * TE_THREADS;
@@ -645,14 +718,25 @@ void launch_sums(const Shape &s, int64_t rows, int64_t dim, int64_t vocab, const
                  const void *dout, int64_t dout_stride, float scale, void *dweight, float *part,
                  hipStream_t stream) {
   constexpr int N = 16 / sizeof(D);
+  const int64_t parts = tv_cdiv(dim, N);
 #define TE_NG(n, g) \
   launch_sums_ng<D, W, n, g>(s, rows, dim, vocab, sorted, dout, dout_stride, scale, dweight, part, stream)
-  const int64_t parts = tv_cdiv(dim, N);
   if (dim < N) TE_NG(1, 16);
   else if (parts <= 16) TE_NG(N, 16);
   else if (parts <= 32) TE_NG(N, 32);
   else TE_NG(N, 64);
 #undef TE_NG
+}
+
+template <typename D, typename W>
+void launch_tiny(int64_t rows, int64_t dim, int64_t vocab, int64_t padding, const int64_t *ids, const void *dout,
+                 int64_t dout_stride, float scale, void *dweight, hipStream_t stream) {
+  constexpr int N = 16 / sizeof(D);
+  const dim3 grid((unsigned)tv_cdiv(vocab, 16 * (TE_THREADS / 64)),
+                  (unsigned)(dim < N ? 1 : tv_cdiv(tv_cdiv(dim, N), 64)));
+  auto kernel = dim < N ? tiny_sums_kernel<D, W, 1> : tiny_sums_kernel<D, W, N>;
+  hipLaunchKernelGGL(kernel, grid, dim3(TE_THREADS), 0, stream, (int)rows, dim, vocab, padding, ids, (const D *)dout,
+                     dout_stride, scale, (W *)dweight);
 }
 
 // (table, rows) types: equal, or an fp32 table with 16-bit rows
@@ -692,7 +776,7 @@ extern "C" int tv_scaled_embedding_fwd(int64_t rows, int64_t dim, int64_t num_to
 
 extern "C" int64_t tv_scaled_embedding_bwd_workspace_bytes(int64_t rows, int64_t dim, int64_t num_tokens) {
   if (!sizes_ok(rows, dim, num_tokens)) return -1;
-  return rows == 0 ? 0 : shape_of(rows, dim, num_tokens).bytes;
+  return rows <= TE_TINY ? 0 : shape_of(rows, dim, num_tokens).bytes;
 }
 
 extern "C" int tv_scaled_embedding_bwd(int64_t rows, int64_t dim, int64_t num_tokens, int weight_dtype,
@@ -710,7 +794,7 @@ extern "C" int tv_scaled_embedding_bwd(int64_t rows, int64_t dim, int64_t num_to
              "tv_scaled_embedding_bwd: misaligned pointer");
   hipStream_t st = (hipStream_t)stream;
   const Shape s = shape_of(rows, dim, num_tokens);
-  if (rows > 0) {
+  if (rows > TE_TINY) {
     TV_REQUIRE(workspace, "tv_scaled_embedding_bwd: null workspace");
     if (workspace_bytes < s.bytes) {
       tv_set_error("tv_scaled_embedding_bwd: workspace too small");
@@ -730,18 +814,29 @@ extern "C" int tv_scaled_embedding_bwd(int64_t rows, int64_t dim, int64_t num_to
     TV_LAUNCH_CHECK("tv_scaled_embedding_bwd");
     return TV_OK;
   }
+#define TE_GO_ALL                                                                           \
+  if (weight_dtype == TV_DTYPE_F32 && out_dtype == TV_DTYPE_F32) TE_GO(float, float);       \
+  else if (weight_dtype == TV_DTYPE_F32 && out_dtype == TV_DTYPE_BF16) TE_GO(__bf16, float); \
+  else if (weight_dtype == TV_DTYPE_F32) TE_GO(_Float16, float);                            \
+  else if (weight_dtype == TV_DTYPE_BF16) TE_GO(__bf16, __bf16);                            \
+  else TE_GO(_Float16, _Float16)
+  if (rows <= TE_TINY) {
+#define TE_GO(D, W) \
+  launch_tiny<D, W>(rows, dim, num_tokens, padding_id, ids, dout, dout_stride, scale, dweight, st)
+    TE_GO_ALL;
+#undef TE_GO
+    TV_LAUNCH_CHECK("tv_scaled_embedding_bwd");
+    return TV_OK;
+  }
   char *ws = (char *)workspace;
   launch_sort(s, rows, Keys{ids, nullptr, num_tokens, padding_id}, ws, st);
   TV_LAUNCH_CHECK("tv_scaled_embedding_bwd");
   const uint2 *sorted = (const uint2 *)(ws + s.pairs0);
   float *part = (float *)(ws + s.part);
 #define TE_GO(D, W) launch_sums<D, W>(s, rows, dim, num_tokens, sorted, dout, dout_stride, scale, dweight, part, st)
-  if (weight_dtype == TV_DTYPE_F32 && out_dtype == TV_DTYPE_F32) TE_GO(float, float);
-  else if (weight_dtype == TV_DTYPE_F32 && out_dtype == TV_DTYPE_BF16) TE_GO(__bf16, float);
-  else if (weight_dtype == TV_DTYPE_F32) TE_GO(_Float16, float);
-  else if (weight_dtype == TV_DTYPE_BF16) TE_GO(__bf16, __bf16);
-  else TE_GO(_Float16, _Float16);
+  TE_GO_ALL;
 #undef TE_GO
+#undef TE_GO_ALL
   TV_LAUNCH_CHECK("tv_scaled_embedding_bwd");
   return TV_OK;
 }

@@ -11,6 +11,7 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <string>
@@ -56,8 +57,8 @@ void *stream_of(const at::Tensor &t) {
   return (void *)c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream();
 }
 
-// what tracevae_amd.ops.scaled_embedding has checked: a [tokens, dim] table with contiguous rows,
-// contiguous int64 ids on its device, types that go together
+// (behind the checks of scaled_embedding below: a [tokens, dim] table with contiguous rows, contiguous
+// int64 ids on its device, types that go together)
 at::Tensor lookup(const at::Tensor &weight, const at::Tensor &ids, double scale, int64_t padding_id, int64_t out_code) {
   const c10::DeviceGuard guard(weight.device());
   const int64_t tokens = weight.size(0), dim = weight.size(1), rows = ids.numel();
@@ -150,6 +151,8 @@ template <typename F> PyObject *guarded(F f) {
     PyErr_SetString(library_error, e.what());
   } catch (const Mismatch &e) {
     PyErr_SetString(PyExc_TypeError, e.what());
+  } catch (const std::invalid_argument &e) {
+    PyErr_SetString(PyExc_ValueError, e.what());
   } catch (const python_error &) {
     // (set already)
   } catch (const c10::OutOfMemoryError &e) {
@@ -160,25 +163,42 @@ template <typename F> PyObject *guarded(F f) {
   return nullptr;
 }
 
+// scaled_embedding(weight, ids, scale, padding_idx or None, out_dtype or None)
 PyObject *scaled_embedding(PyObject *, PyObject *const *args, Py_ssize_t n) {
-  if (n != 5 || !THPVariable_Check(args[0]) || !THPVariable_Check(args[1])) {
-    PyErr_SetString(PyExc_TypeError, "scaled_embedding(weight, ids, scale, padding_id, out_dtype)");
+  if (n != 5 || !THPVariable_Check(args[0]) || !THPVariable_Check(args[1]) ||
+      !(args[4] == Py_None || THPDtype_Check(args[4]))) {
+    PyErr_SetString(PyExc_TypeError, "scaled_embedding(weight, ids, scale, padding_idx, out_dtype): two tensors, "
+                                     "a number, a number or None, a torch.dtype or None");
     return nullptr;
   }
   const double scale = PyFloat_AsDouble(args[2]);
-  const int64_t padding = PyLong_AsLongLong(args[3]), out_code = PyLong_AsLongLong(args[4]);
+  const int64_t padding = args[3] == Py_None ? -1 : PyLong_AsLongLong(args[3]);
   if (PyErr_Occurred()) return nullptr;
   return guarded([&]() -> PyObject * {
-    const at::Tensor &weight = THPVariable_Unpack(args[0]), &ids = THPVariable_Unpack(args[1]);
+    at::Tensor weight = THPVariable_Unpack(args[0]), ids = THPVariable_Unpack(args[1]);
+    if (!weight.is_cuda() || ids.device() != weight.device())
+      throw LibraryError("weight is on " + weight.device().str() + ", ids on " + ids.device().str() +
+                         ": the accelerated path runs on the GPU only (there is no CPU fallback)");
+    const at::ScalarType in = weight.scalar_type();
+    const at::ScalarType to = args[4] == Py_None ? in : reinterpret_cast<THPDtype *>(args[4])->scalar_type;
+    if (dtype_code(in) < 0 || dtype_code(to) < 0 || (to != in && in != at::kFloat))
+      throw Mismatch(std::string("a table of ") + c10::toString(in) + " does not give rows of " + c10::toString(to));
+    if (ids.scalar_type() != at::kLong)
+      throw Mismatch(std::string("ids must be torch.int64, got ") + c10::toString(ids.scalar_type()));
+    if (weight.layout() != at::kStrided || ids.layout() != at::kStrided) throw Mismatch("weight and ids are dense");
+    if (weight.dim() != 2 || weight.numel() == 0) throw std::invalid_argument("weight must be [tokens, dim]");
     at::Tensor out;
     {
       struct Released {                           // (also when an exception passes)
         PyThreadState *state = PyEval_SaveThread();
         ~Released() { PyEval_RestoreThread(state); }
       } released;
+      if (!weight.is_contiguous() && (weight.stride(1) != 1 || weight.stride(0) < weight.size(1)))
+        weight = weight.contiguous();
+      ids = ids.contiguous();
       out = at::GradMode::is_enabled() && weight.requires_grad()
-                ? ScaledEmbedding::apply(weight, ids, scale, padding, out_code)
-                : lookup(weight, ids, scale, padding, out_code);
+                ? ScaledEmbedding::apply(weight, ids, scale, padding, dtype_code(to))
+                : lookup(weight, ids, scale, padding, dtype_code(to));
     }
     return THPVariable_Wrap(out);
   });

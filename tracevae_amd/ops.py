@@ -1219,35 +1219,14 @@ def embedding(weight, ids, extra_cols: int = 0):
     return _Embedding.apply(weight, ids, extra_cols)
 
 
-_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # TV_DTYPE_*
-
-
 def scaled_embedding(weight, ids, scale: float = 1.0, padding_idx: Optional[int] = None,
                      out_dtype: Optional[torch.dtype] = None):
     """`scale * weight[ids]`, rounded once to `out_dtype` (default: the table's type; a 16-bit type
-    for an fp32 table), of shape `ids.shape + (dim,)`.  Ids outside the table and `padding_idx` give
-    rows of zeros and no gradient.  The gradient of the table is summed in fp32 over its tokens in
+    for an fp32 table), of shape `ids.shape + (dim,)`.  Ids outside the table and ids equal to
+    `padding_idx` (which is not counted from the end) give rows of zeros and no gradient.  The gradient of the table is summed in fp32 over its tokens in
     the order of `ids`, whatever their number (`tv_scaled_embedding_bwd`), and is dense.
     `weight`: [tokens, dim] in fp32, bf16 or fp16 with contiguous, possibly strided rows."""
-    if not weight.is_cuda or ids.device != weight.device:
-        raise hip.HipLibraryError(f'weight is on {weight.device}, ids on {ids.device}: the accelerated '
-                                  f'path runs on the GPU only (there is no CPU fallback)')
-    dtype = weight.dtype
-    if out_dtype is None:
-        out_dtype = dtype
-    if dtype not in _DTYPES or out_dtype not in _DTYPES \
-            or (out_dtype != dtype and dtype != torch.float32):
-        raise TypeError(f'a table of {dtype} does not give rows of {out_dtype}')
-    if ids.dtype != torch.int64:
-        raise TypeError(f'ids must be torch.int64, got {ids.dtype}')
-    if not weight.is_contiguous():
-        if weight.dim() == 2 and (weight.stride(1) != 1 or weight.stride(0) < weight.shape[1]):
-            weight = weight.contiguous()
-    if weight.dim() != 2 or weight.numel() == 0:
-        raise ValueError(f'weight must be [tokens, dim], got {tuple(weight.shape)}')
-    return hip.host().scaled_embedding(weight, ids if ids.is_contiguous() else ids.contiguous(),
-                                       scale, -1 if padding_idx is None else padding_idx,
-                                       _DTYPES[out_dtype])
+    return hip.host().scaled_embedding(weight, ids, scale, padding_idx, out_dtype)
 
 
 class _LatDecInput(Function):

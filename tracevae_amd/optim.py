@@ -19,8 +19,8 @@ BLOCK = 256                                                            # TV_ADAM
 
 
 class AdamW(object):
-    """One AdamW step over all of `params` per `step()`: three launches with clipping, two without
-    (one or two more for every 384 tensors).
+    """One AdamW step over all of `params` per `step()`: three launches with clipping, two without,
+    one for few tensors without clipping and guard (one or two more for every 384 tensors).
 
         m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2
         p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
@@ -122,9 +122,15 @@ class AdamW(object):
                         ctypes.addressof(where), self._decay,
                         image.data_ptr(), nbytes)
         self._plan_host, self._plan, self._where = image, image.to(self.device), where
-        self._arrays = tuple(ctypes.addressof(x) for x in (self._dtypes, self._sizes, self._where,
-                                                           self._addresses))
-        self._plan_at = (self._plan_host.data_ptr(), self._plan.data_ptr())
+        # the arguments of a step that stay the same: the optimizer's own arrays and buffers
+        names = ('exp_avg', 'exp_avg_sq', None, None) if self.state_bits == 32 else \
+            ('exp_avg8', 'exp_rms8', 'exp_avg_scale', 'exp_rms_scale')
+        self._fixed = tuple(ctypes.addressof(x) for x in (self._dtypes, self._sizes, self._where,
+                                                          self._addresses)) + \
+            (self._plan_host.data_ptr(), self._plan.data_ptr(), self.state_bits) + \
+            tuple(None if n is None else self._state[n].data_ptr() for n in names) + \
+            (self._state['master'].data_ptr() if 'master' in self._state else None,
+             self._control.data_ptr())
 
     # -- hyper-parameters and state ----------------------------------------------------
     def set_lr(self, lr: float) -> None:
@@ -179,18 +185,12 @@ class AdamW(object):
         if guard_host is not None and (guard_host.dtype != torch.float32 or guard_host.numel() != 1
                                        or guard_host.is_cuda):
             raise TypeError('guard_host must be one float32 in pinned host memory')
-        s, clip = self._state, float(global_clip_norm or 0.0)
-        if self.state_bits == 32:
-            moments = (s['exp_avg'].data_ptr(), s['exp_avg_sq'].data_ptr(), None, None)
-        else:
-            moments = (s['exp_avg8'].data_ptr(), s['exp_rms8'].data_ptr(),
-                       s['exp_avg_scale'].data_ptr(), s['exp_rms_scale'].data_ptr())
+        clip = float(global_clip_norm or 0.0)
         if grads is not None and type(grads) is not list:
             grads = list(grads)
         step = hip.host().adamw_step
-        while not step(self.params, grads, *self._arrays, *self._plan_at, self.state_bits, *moments,
-                       s['master'].data_ptr() if 'master' in s else None, self._control.data_ptr(),
-                       clip, self.grad_norm.data_ptr() if clip else None, self.seed, hip.ptr(guard),
+        while not step(self.params, grads, *self._fixed, clip,
+                       self.grad_norm.data_ptr() if clip else None, self.seed, hip.ptr(guard),
                        guard_kind if guard is not None else 0,
                        guard_host.data_ptr() if guard_host is not None else None,
                        self._workspace.data_ptr(), self._workspace.numel() * 8, hip.stream(),
