@@ -733,13 +733,12 @@ int tv_optim_step_guarded(int kind, int64_t n, float *param, const float *grad, 
  * caller-owned, 16-byte aligned, zero before the first step:
  *   state_bits 32: moment1 = m, moment2 = v, fp32; scales NULL
  *   state_bits  8: moment1 = m / scale1, moment2 = sqrt(v) / scale2, one e4m3 byte each, one fp32
- *     scale per TV_ADAMW_BLOCK elements = (largest finite magnitude of the block) * fp32(1/448).  Codes
- *     are
- *     rounded up or down with the probabilities that keep the value on average, by a hash of
- *     (seed, step, element): same seed, same bits.  A positive sqrt(v) keeps a positive code; an
- *     infinite or NaN moment becomes the NaN code and leaves its neighbours alone; a block whose
- *     scale would be below 2^-126 is stored as zeros.  Everything up to codes and scales is float64,
- *     m as two products and a sum, each rounded.
+ *     scale per TV_ADAMW_BLOCK elements = (largest finite magnitude of the block) * fp32(1/448).
+ *     Codes are rounded up or down with the probabilities that keep the value on average, by a hash
+ *     of (seed, step, element): same seed, same bits.  A sqrt(v) that is positive in fp32 keeps a
+ *     positive code; an infinite or NaN moment becomes the NaN code and leaves its neighbours alone;
+ *     a block whose scale would be below 2^-100 is stored as zeros.  Everything up to codes and scales
+ *     is float64, m as two products and a sum, each rounded.
  *   master: fp32, needed if any parameter has 16 bits (otherwise NULL).
  *
  * tv_adamw_plan writes the table of tensors and chunks into HOST memory; the caller keeps it and a

@@ -27,14 +27,14 @@ def to_codes(x, random16, positive):
     finite = torch.isfinite(x)
     mag = torch.where(finite, x.abs(), 0.0)
     scale = mag.amax(1, keepdim=True).float() * torch.tensor(1 / 448, dtype=torch.float32)
-    scale = torch.where(scale >= 2.0 ** -126, scale, torch.zeros_like(scale))
+    scale = torch.where(scale >= 2.0 ** -100, scale, torch.zeros_like(scale))
     y = torch.where(scale > 0, mag / scale.double(), 0.0).clamp(max=448.0)
     at = torch.searchsorted(GRID, y.contiguous(), right=True) - 1
     above = torch.cat([GRID[1:], GRID[-1:]])
     gap = (above[at] - GRID[at]).clamp(min=1e-300)
     q = torch.where((y - GRID[at]) / gap + (random16.double() + 0.5) / 65536 >= 1, above[at], GRID[at])
     if positive:
-        q = torch.where((mag > 0) & (q == 0), GRID[1], q)
+        q = torch.where((mag.float() > 0) & (q == 0), GRID[1], q)
     return torch.where(finite, torch.copysign(q, x), math.nan), scale
 
 

@@ -116,6 +116,9 @@ class Twin(object):
                 assert torch.equal(s[name + '_scale'][hb], scale.view(-1)[hb])
                 assert torch.equal(s[name + '8'].double().view(-1, 256)[hb], q[hb])
             bound = 3 * U * (p0.abs() + change.abs()) + 8 * U * change.abs()
+        # below 2^-126 fp32 has steps of 2^-149 whatever the value: in m, times what it is multiplied by,
+        # in the quotient, times the step size, and in the result
+        bound = bound + 2.0 ** -149 * (size + opt.lr / (1 - b1 ** self.t) + 1)
         assert ((got_p - p1).abs() <= bound)[has].all()
         # what has no gradient, and what lies between tensors, is as it was
         for k, v in s.items():
@@ -251,6 +254,22 @@ def test_extreme_gradients(device, bits):
     assert torch.allclose(params[0], before[0] * (1 - 1e-2 * 0.01) ** 3, rtol=1e-6, atol=0)
     moved = (params[2] - before[2] * (1 - 1e-2 * 0.01) ** 3)
     assert ((moved + 3e-2).abs() < 3e-2 * 0.15).all()       # 8 bits: m and r are within 1/8 of theirs
+
+
+def test_codes_of_tiny_and_mixed_magnitudes(device):
+    """Blocks from 1e-36 to 1e15 in size, each with elements over 12 decades, zeros among them, and blocks
+    of nothing but zeros: codes and scales equal to the definition's."""
+    from tracevae_amd.optim import AdamW
+    gen = torch.Generator().manual_seed(3)
+    params = [torch.zeros(200, 256, device=device), torch.zeros(300, device=device)]
+    opt = AdamW(params, weight_decay=0.0, state_bits=8, seed=9, **HYPER)
+    twin = Twin(opt, [0.0, 0.0])
+    for k in range(3):
+        size = 10.0 ** torch.linspace(-36, 15, 200).view(-1, 1)
+        g = torch.randn(200, 256, generator=gen) * size * 10.0 ** (-12 * torch.rand(200, 256, generator=gen))
+        g[torch.rand(200, 256, generator=gen) < 0.2] = 0.0
+        g[::7] = 0.0
+        twin.step([g.to(device), torch.zeros(300, device=device)])
 
 
 @pytest.mark.parametrize('bits', [32, 8])

@@ -302,20 +302,20 @@ __host__ __device__ inline uint32_t mix(uint32_t x) {
   return x ^ (x >> 16);
 }
 
-// e4m3 magnitude code of y in [0, 448 (1 + 2^-23)], rounded up with the probability of what is left
-// over the code below: 17 random bits (the lowest always set, so an exact value stays) are added to
-// the 17 mantissa bits of the high word that e4m3 drops.  Below 2^-6 codes lie 2^-9 apart: adding
-// 2^-6 puts those bits at the same place.
-__device__ __forceinline__ uint32_t code_of(double y, uint32_t random16) {
-  const bool low = y < 0.015625;
-  const double z = low ? y + 0.015625 : y;
-  const uint32_t hi = (uint32_t)__double2hiint(z) + (2 * random16 + 1);
-  const uint32_t c = (hi >> 17) - (1016u << 3) - (low ? 8u : 0u);
+// e4m3 magnitude code of y = x / scale in [0, 448 (1 + 2^-23)], rounded up with the probability of what
+// is left over the code below: 17 random bits (the lowest always set, so an exact value stays) are added
+// to the 17 mantissa bits of the high word that e4m3 drops.  Below 2^-6 codes lie 2^-9 apart: adding 2^-6
+// puts those bits at the same place.  `low` may be decided in fp32: within 2^-22 of 2^-6 both ways give
+// the code of 2^-6.
+__device__ __forceinline__ uint32_t code_of(double x, double inverse_scale, bool low, uint32_t random17) {
+  const double z = fma(x, inverse_scale, __hiloint2double(low ? 0x3f900000 : 0, 0));
+  const uint32_t base = low ? 1017u << 20 : 1016u << 20;
+  const uint32_t c = ((uint32_t)__double2hiint(z) + random17 - base) >> 17;
   return c < 126u ? c : 126u;
 }
 __device__ __forceinline__ float scale_of(float largest) {
   const float s = largest * (1.f / 448.f);
-  return s >= 1.17549435e-38f ? s : 0.f;          // (below that the block counts as zero)
+  return s >= 0x1p-100f ? s : 0.f;                // (below that the block counts as zero)
 }
 __device__ __forceinline__ void decode4(uint32_t c, float (&x)[4]) {
   typedef float F2 __attribute__((ext_vector_type(2)));
@@ -324,9 +324,9 @@ __device__ __forceinline__ void decode4(uint32_t c, float (&x)[4]) {
   x[0] = a[0]; x[1] = a[1]; x[2] = b[0]; x[3] = b[1];
 }
 
-// largest value of a wave, of values that are not negative: their bits compare as integers
-__device__ __forceinline__ float wave_largest(float x) {
-  uint32_t v = __float_as_uint(x);
+constexpr uint32_t INF_BITS = 0x7f800000u;
+// largest value of a wave
+__device__ __forceinline__ uint32_t wave_largest(uint32_t v) {
 #define AW_DPP(ctrl) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, 0xf, 0xf, false))
   AW_DPP(0x111);   // row_shr 1, 2, 4, 8: lane 15 of each row of 16 has the row's
   AW_DPP(0x112);
@@ -335,7 +335,7 @@ __device__ __forceinline__ float wave_largest(float x) {
   AW_DPP(0x142);   // row_bcast 15, 31: lane 63 has the wave's
   AW_DPP(0x143);
 #undef AW_DPP
-  return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)v, 63));
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 
 // a b + c d, each of the three rounded.  (b1 m + (1 - b1) g with b1 = 0.9 is (9 m + g) / 10: one in some
@@ -346,22 +346,17 @@ __device__ __forceinline__ double two_products(double a, double b, double c, dou
   const double x = a * b, y = c * d;
   return x + y;
 }
-// sqrt(v): an fp32 estimate and two Newton steps (2^-23, 2^-45, then the rounding of float64; the
-// library's sqrt is twice as long).  One step is not enough: the largest root of a block is rounded to
-// fp32 for its scale, and 2^-45 decides one such rounding in 2 million.
+// sqrt(v) for v > 0 to 2^-47 (NaN for inf): the hardware's reciprocal root (2^-24) and one Newton step, a
+// third of the library's sqrt.  (That is enough for the codes; the fp32 scale, made from the largest root
+// of a block, is the neighbouring number in one block of some 10 million.  A second step costs 2 % of the
+// whole.)
 __device__ __forceinline__ double root(double v) {
-  const float f = (float)v;
-  if (f > 1e-30f && f < 1e30f) {
-    const double q = (double)__builtin_amdgcn_rsqf(f), h = 0.5 * q;
-    double r = v * q;
-    r = fma(fma(-r, r, v), h, r);
-    return fma(fma(-r, r, v), h, r);
-  }
-  return v == 0.0 ? 0.0 : sqrt(v);
+  const double q = __builtin_amdgcn_rsq(v), r = v * q;
+  return fma(fma(-r, r, v), 0.5 * q, r);
 }
 // 1 / s to 2^-45, 0 for 0
 __device__ __forceinline__ double inverse(float s) {
-  if (s > 1e-30f && s < 1e30f) {
+  if (s > 0.f && s < 1e30f) {                     // (at least 2^-100)
     const double d = (double)s, q = (double)__builtin_amdgcn_rcpf(s);
     return fma(fma(-d, q, 1.0), q, q);
   }
@@ -386,34 +381,54 @@ __device__ __forceinline__ void chunk_step8(T *p, const T *g, float *w, uint32_t
     decode4(__builtin_nontemporal_load(r8 + i / 4), ro);
     if (sizeof(T) != 4) load4(w, i, wx);
     const double sm = ms[b], sr = rs[b];
+    const double k2 = s.beta2 * (sr * sr);
     double mx[4], rx[4];
-    float am = 0.f, ar = 0.f;
+    uint32_t am = 0, ar = 0;                      // bits of the largest |m| and rms in fp32
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const double gj = (double)gx[j] * s.coef;
-      const double ro_ = ro[j] * sr;
       mx[j] = two_products(s.beta1, mo[j] * sm, s.omb1, gj);
-      rx[j] = root(fma(s.beta2, ro_ * ro_, s.omb2 * gj * gj));
-      const float mf = fabsf((float)mx[j]), rf = (float)rx[j];
-      if (mf < INFINITY) am = fmaxf(am, mf);
-      if (rf < INFINITY) ar = fmaxf(ar, rf);
+      // (the square of a code has 8 bits: exact in fp32.  1e-300 keeps a zero from 0 / 0: its root is zero
+      // in fp32, and gradients that are not zero have squares above 1e-90)
+      rx[j] = root(fma(k2, (double)(ro[j] * ro[j]), fma(s.omb2 * gj, gj, 1e-300)));
+      am = max(am, __float_as_uint(fabsf((float)mx[j])));
+      ar = max(ar, __float_as_uint(fabsf((float)rx[j])));
     }
-    const float nm = scale_of(wave_largest(am)), nr = scale_of(wave_largest(ar));
+    am = wave_largest(am);
+    ar = wave_largest(ar);
+    const bool odd = max(am, ar) >= INF_BITS;     // (the same for the whole wave)
+    if (odd) {                                    // infinite or NaN moments: the scales are the others'
+      am = ar = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t mb = __float_as_uint(fabsf((float)mx[j])), rb = __float_as_uint(fabsf((float)rx[j]));
+        am = max(am, mb < INF_BITS ? mb : 0u);
+        ar = max(ar, rb < INF_BITS ? rb : 0u);
+      }
+      am = wave_largest(am);
+      ar = wave_largest(ar);
+    }
+    const float nm = scale_of(__uint_as_float(am)), nr = scale_of(__uint_as_float(ar));
     const double im = inverse(nm), ir = inverse(nr);
+    // below 2^-6 of a scale; everything in a block of zeros
+    const float lm = nm > 0.f ? nm * 0.015625f : INFINITY, lr = nr > 0.f ? nr * 0.015625f : INFINITY;
     uint32_t cm = 0, cr = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const uint32_t u = mix(key ^ (element + (uint32_t)j));
       const float mf = (float)mx[j], rf = (float)rx[j];
-      uint32_t a = code_of(fabs(mx[j]) * im, u & 0xffffu);
-      uint32_t c = code_of(rx[j] * ir, u >> 16);
-      c = rf > 0.f ? max(c, 1u) : c;              // a positive rms stays positive
-      a = fabsf(mf) < INFINITY ? a : 127u;        // NaN
-      c = rf < INFINITY ? c : 127u;
-      a |= (__float_as_uint(mf) >> 24) & 0x80u;
-      cm |= a << (8 * j);
-      cr |= c << (8 * j);
+      const uint32_t a = code_of(fabs(mx[j]), im, fabsf(mf) < lm, ((u << 1) & 0x1ffffu) | 1u);
+      const uint32_t c = code_of(rx[j], ir, rf < lr, (u >> 15) | 1u);
+      cm |= (a | ((__float_as_uint(mf) >> 24) & 0x80u)) << (8 * j);
+      cr |= max(c, min(__float_as_uint(rf), 1u)) << (8 * j);      // a positive rms stays positive
       px[j] = moved8(sizeof(T) == 4 ? px[j] : master_of<T>(px[j], wx[j]), mf, rf, s);
+    }
+    if (__builtin_expect(odd, 0)) {               // infinite and NaN moments become NaN
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (__float_as_uint(fabsf((float)mx[j])) >= INF_BITS) cm |= 0x7fu << (8 * j);
+        if (__float_as_uint(fabsf((float)rx[j])) >= INF_BITS) cr |= 0x7fu << (8 * j);
+      }
     }
     store4(p, i, n, px);
     if (sizeof(T) != 4) store_master(w, i, n, px);
