@@ -80,6 +80,9 @@ __host__ __device__ inline const Chunk *plan_chunks(const void *plan, int64_t co
 // without: 14 million parameters 82 us against 95 (32 bits), 60 against 68 (8 bits), 343 million
 // 1.96 ms against 2.11 and 1.01 against 1.06.  (One model stepped over and over, whose 228 MB stay in
 // the 256 MB last-level cache, takes 64 us with it and 60 without.)
+// Parameters and gradients come by addresses out of memory, which the compiler takes for generic ones
+// (flat accesses, which wait for LDS as well): they are global.
+#define AW_GLOBAL __attribute__((address_space(1)))
 template <typename T> struct Four {                // four elements, at any alignment of the type
   typedef T V __attribute__((ext_vector_type(4)));
   typedef V Any __attribute__((aligned(sizeof(T))));
@@ -87,28 +90,30 @@ template <typename T> struct Four {                // four elements, at any alig
 // four consecutive elements from i on, zeros behind n
 template <typename T>
 __device__ __forceinline__ void load4(const T *p, int i, int n, float (&x)[4]) {
+  const AW_GLOBAL T *q = (const AW_GLOBAL T *)(p + i);
   if (i + 4 <= n) {
     typedef typename Four<T>::Any Any;
-    const typename Four<T>::V f = __builtin_nontemporal_load(reinterpret_cast<const Any *>(p + i));
+    const typename Four<T>::V f = __builtin_nontemporal_load((const AW_GLOBAL Any *)q);
 #pragma unroll
     for (int j = 0; j < 4; ++j) x[j] = (float)f[j];
   } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = i + j < n ? (float)p[i + j] : 0.f;
+    for (int j = 0; j < 4; ++j) x[j] = i + j < n ? (float)q[j] : 0.f;
   }
 }
 template <typename T>
 __device__ __forceinline__ void store4(T *p, int i, int n, const float (&x)[4]) {
+  AW_GLOBAL T *q = (AW_GLOBAL T *)(p + i);
   if (i + 4 <= n) {
     typedef typename Four<T>::Any Any;
     typename Four<T>::V f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) f[j] = (T)x[j];
-    __builtin_nontemporal_store(f, reinterpret_cast<Any *>(p + i));
+    __builtin_nontemporal_store(f, (AW_GLOBAL Any *)q);
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (i + j < n) p[i + j] = (T)x[j];
+      if (i + j < n) q[j] = (T)x[j];
   }
 }
 // the state: 16-byte aligned segments, padded to 256 elements
@@ -137,13 +142,16 @@ template <typename T> __device__ __forceinline__ double chunk_sumsq(const T *g, 
     typename Four<T>::V x[AW_ITS];                  // (without the hint: the step reads them again)
 #pragma unroll
     for (int it = 0; it < AW_ITS; ++it)
-      x[it] = *reinterpret_cast<const typename Four<T>::Any *>(g + it * 4 * AW_THREADS + (int)threadIdx.x * 4);
+      x[it] = *(const AW_GLOBAL typename Four<T>::Any *)(g + it * 4 * AW_THREADS + (int)threadIdx.x * 4);
 #pragma unroll
     for (int it = 0; it < AW_ITS; ++it)
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc = fma((double)(float)x[it][j], (double)(float)x[it][j], acc);
   } else {
-    for (int i = (int)threadIdx.x; i < n; i += AW_THREADS) acc = fma((double)(float)g[i], (double)(float)g[i], acc);
+    for (int i = (int)threadIdx.x; i < n; i += AW_THREADS) {
+      const double x = (double)(float)((const AW_GLOBAL T *)g)[i];
+      acc = fma(x, x, acc);
+    }
   }
   return acc;
 }
@@ -502,15 +510,16 @@ __global__ __launch_bounds__(AW_THREADS) void adamw_step_kernel(
     }
   }
   if (ALONE) {
-    __syncthreads();                              // the whole workgroup has read the counters
-    if (threadIdx.x == 0) {
-      __threadfence();
-      if (atomicAdd(&ctl->ticket, 1u) == gridDim.x * gridDim.y - 1) {
-        ctl->ticket = 0;
-        ctl->step = step;
-        ctl->beta1_t = b1t;
-        ctl->beta2_t = b2t;
-      }
+    // Behind the barrier the whole workgroup has its copy of the counters, and thread 0 has used its own;
+    // the last ticket so means that nobody reads them any more.  No fence to the device: nothing that
+    // this workgroup has written is read in this launch (and such a fence writes the L2 back: 2 us).
+    __syncthreads();
+    if (threadIdx.x == 0 && __hip_atomic_fetch_add(&ctl->ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+                                gridDim.x * gridDim.y - 1) {
+      ctl->ticket = 0;
+      ctl->step = step;
+      ctl->beta1_t = b1t;
+      ctl->beta2_t = b2t;
     }
   }
 }
