@@ -363,3 +363,38 @@ def test_table_trained_by_lookup_gradient_and_adamw(device, bits, capture):
                 q, scale = ref.to_codes(x.view(-1, 256), u, name == 'exp_rms')
                 assert torch.equal(opt.state[name + '_scale'].cpu(), scale.view(-1))
                 assert torch.equal(opt.state[name + '8'].cpu().double().view(-1, 256), q)
+
+
+def test_backward_accumulates_and_the_optimizer_reads_grad(device):
+    """The loop of a user's program: .backward() twice into .grad, step(), zero_grad(); tensors of three
+    types in one optimizer, gradients by autograd."""
+    from tracevae_amd import AdamW, ops
+    gen = torch.Generator().manual_seed(12)
+    table = torch.nn.Parameter((torch.randn(300, 32, generator=gen) * 0.1).to(device))
+    half = torch.nn.Parameter((torch.randn(300, 32, generator=gen) * 0.1).half().to(device))
+    head = torch.nn.Linear(32, 5).to(device).bfloat16()
+    unused = torch.nn.Parameter(torch.ones(7, device=device))
+    opt = AdamW([table, half, *head.parameters(), unused], lr=1e-2, weight_decay=0.0, state_bits=8)
+    ids = torch.randint(-1, 300, (6, 50), generator=gen).to(device)
+    grads = []
+    for _ in range(2):
+        a = ops.scaled_embedding(table, ids, 2.0, out_dtype=torch.bfloat16)
+        b = ops.scaled_embedding(half, ids, 2.0)
+        (head(a).float().square().mean() + b.float().square().sum()).backward()
+        grads.append([p.grad.clone() for p in (table, half, *head.parameters())])
+    for first, both in zip(*grads):
+        assert torch.allclose(both.float(), 2 * first.float(), rtol=1e-2, atol=1e-6)
+    before = [p.detach().clone() for p in opt.params]
+    version = table._version
+    norm = opt.step(global_clip_norm=1.0)
+    want = math.sqrt(sum(float(g.double().square().sum()) for g in grads[1]))
+    assert abs(float(norm) - want) <= 2.0 ** -40 * want
+    assert table._version > version                       # autograd knows that it was written
+    for p, q in zip(opt.params, before):
+        assert torch.equal(p, q) == (p is unused)
+        assert torch.isfinite(p).all()
+    named = torch.zeros(300, dtype=torch.bool)
+    named[ids.cpu().reshape(-1)[ids.cpu().reshape(-1) >= 0]] = True
+    assert torch.equal(table.detach().cpu()[~named], before[0].cpu()[~named])     # rows nobody named
+    opt.zero_grad()
+    assert all(p.grad is None for p in opt.params)

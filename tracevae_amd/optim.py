@@ -167,6 +167,11 @@ class AdamW(object):
             v.view(torch.uint8).copy_(state[k].to(self.device).contiguous().view(torch.uint8))
         self._write_control(int(state['step']))
 
+    def zero_grad(self) -> None:
+        """Drops the gradients (the next backward pass hands over fresh ones)."""
+        for p in self.params:
+            p.grad = None
+
     # -- one step ----------------------------------------------------------------------
     def step(self, grads: Optional[Sequence[Optional[torch.Tensor]]] = None,
              global_clip_norm: Optional[float] = None, guard: Optional[torch.Tensor] = None,
