@@ -332,6 +332,7 @@ def test_captured_step_counts_on(device, bits, clip):
 
 
 def test_state_dict_continues_bit_for_bit(device):
+    from tracevae_amd.hip import HipLibraryError
     from tracevae_amd.optim import AdamW
     for bits in (32, 8):
         params = _params(ODD, torch.float16, device, 16)
@@ -350,6 +351,11 @@ def test_state_dict_continues_bit_for_bit(device):
             AdamW(copies, state_bits=40 - bits, **HYPER).load_state_dict(saved)
         with pytest.raises(ValueError):
             AdamW(copies[:3], state_bits=bits, **HYPER).load_state_dict(saved)
+        with pytest.raises(HipLibraryError):
+            again.load_state_dict(dict(saved, step=-1))
+        assert again.steps == 3
+        for k in opt.state:
+            assert torch.equal(opt.state[k].view(torch.uint8), again.state[k].view(torch.uint8))
 
 
 def test_the_master_follows_a_weight_that_was_written(device):

@@ -171,6 +171,17 @@ def test_difference_quotient_and_two_uses(device):
     assert torch.equal(w.grad, 2 * dw)
 
 
+def test_one_id_without_a_dimension(device):
+    from tracevae_amd import ops
+    w = torch.randn(9, 20, device=device, requires_grad=True)
+    out = ops.scaled_embedding(w, torch.tensor(4, device=device), 2.0)
+    assert out.shape == (20,) and torch.equal(out, 2 * w[4])
+    (dw,) = torch.autograd.grad(out, w, torch.ones(1, device=device).expand(20))
+    want = torch.zeros(9, 20, device=device)
+    want[4] = 2.0
+    assert torch.equal(dw, want)
+
+
 def test_no_second_derivative_and_no_changed_ids(device):
     from tracevae_amd import ops
     w = torch.randn(50, 16, device=device, requires_grad=True)
@@ -382,8 +393,8 @@ def test_backward_accumulates_and_the_optimizer_reads_grad(device):
         b = ops.scaled_embedding(half, ids, 2.0)
         (head(a).float().square().mean() + b.float().square().sum()).backward()
         grads.append([p.grad.clone() for p in (table, half, *head.parameters())])
-    for first, both in zip(*grads):
-        assert torch.allclose(both.float(), 2 * first.float(), rtol=1e-2, atol=1e-6)
+    for first, both in zip(*grads):                       # (twice a number is exact)
+        assert torch.equal(both, 2 * first)
     before = [p.detach().clone() for p in opt.params]
     version = table._version
     norm = opt.step(global_clip_norm=1.0)

@@ -32,7 +32,7 @@ class AdamW(object):
     * `state_bits` 32: `state['exp_avg']`, `state['exp_avg_sq']` in fp32.  8: `state['exp_avg8']` and
       `state['exp_rms8']` (torch.float8_e4m3fn; sqrt(v), not v) in units of `state['exp_avg_scale']` /
       `state['exp_rms_scale']`, one fp32 scale per 256 elements; rounded stochastically by a hash of
-      (`seed`, step, element), so a run is reproducible bit for bit.
+      (the low 32 bits of `seed`, step, element), so a run is reproducible bit for bit.
     * all state buffers are flat: tensor i begins at `offsets[i]`, a multiple of 256.
     * the step counter and the learning rate are on the device: `step()` never waits for the GPU and
       may be captured into a graph (capture after the first eager step; `set_lr` between replays is
@@ -99,6 +99,7 @@ class AdamW(object):
         self._write_control(0)
         self._workspace = zeros(int(lib.tv_adamw_workspace_bytes(n)) // 8, torch.float64)
         self.grad_norm = torch.zeros((), dtype=torch.float64, device=self.device)
+        self._plan = None
         self._make_plan()
 
     # -- set-up ------------------------------------------------------------------------
@@ -121,6 +122,9 @@ class AdamW(object):
         self._call_host('tv_adamw_plan', n, self._sizes, self._dtypes,
                         ctypes.addressof(where), self._decay,
                         image.data_ptr(), nbytes)
+        if self._plan is not None:
+            # a step may still read it, on a stream that is not the one it was allocated on
+            self._plan.record_stream(torch.cuda.current_stream(self.device))
         self._plan_host, self._plan, self._where = image, image.to(self.device), where
         # the arguments of a step that stay the same: the optimizer's own arrays and buffers
         names = ('exp_avg', 'exp_avg_sq', None, None) if self.state_bits == 32 else \
@@ -163,9 +167,9 @@ class AdamW(object):
             if tuple(state[k].shape) != tuple(v.shape) or state[k].dtype != v.dtype:
                 raise ValueError(f'{k} must be {v.dtype} of {tuple(v.shape)}, got {state[k].dtype} '
                                  f'of {tuple(state[k].shape)}')
+        self._write_control(int(state['step']))
         for k, v in self._state.items():
             v.view(torch.uint8).copy_(state[k].to(self.device).contiguous().view(torch.uint8))
-        self._write_control(int(state['step']))
 
     def zero_grad(self) -> None:
         """Drops the gradients (the next backward pass hands over fresh ones)."""
