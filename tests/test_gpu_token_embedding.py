@@ -262,6 +262,76 @@ def test_captured_and_replayed(device):
         assert torch.equal(out, want_out.detach()) and torch.equal(dw, want_dw), kind
 
 
+@pytest.mark.parametrize('cast', [False, True])
+def test_a_capture_beside_a_living_eager_graph_is_refused(device, cast):
+    """A captured backward pass that leads to a leaf whose accumulator an eager graph holds is refused while
+    the capture is still sound; without that graph, or up to a tensor made in the capture, it is taken."""
+    from tracevae_amd import ops
+    ids = torch.arange(600, device=device) % 37
+    w = torch.randn(40, 16, device=device, requires_grad=True)
+    dout = torch.randn(600, 16, device=device, dtype=torch.bfloat16 if cast else torch.float32)
+
+    def both(backward):
+        table = w.bfloat16() if cast else w
+        out = ops.scaled_embedding(table, ids, 2.0)
+        return out, backward(out, table)
+
+    want = both(lambda out, table: torch.autograd.grad(out, w, dout)[0])[1]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both(lambda out, table: torch.autograd.grad(out, w, dout)[0])
+    torch.cuda.synchronize()
+    kept = w * 1.0                                        # the eager graph
+    refused = []
+
+    def expect_refusal(backward):
+        def run(out, table):
+            try:
+                backward(out, table)
+            except RuntimeError as e:
+                refused.append('eager graph' in str(e))
+        return run
+
+    for backward in (lambda out, table: torch.autograd.grad(out, w, dout), lambda out, table: out.backward(dout)):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = both(expect_refusal(backward))[0].detach()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, 2 * (w.detach().bfloat16() if cast else w.detach())[ids])
+    assert refused == [True, True] and w.grad is None
+    if cast:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            dw = both(lambda out, table: torch.autograd.grad(out, table, dout)[0])[1].detach()
+        graph.replay()
+        assert torch.equal(dw.float(), want)
+    assert torch.equal(torch.autograd.grad(kept.sum(), w)[0], torch.ones_like(w))
+    del kept
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        dw = both(lambda out, table: torch.autograd.grad(out, w, dout)[0])[1].detach()
+    for _ in range(3):
+        dw.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(dw, want)
+
+
+def test_the_node_called_by_hand_refuses_other_gradients(device):
+    from tracevae_amd import ops
+    w = torch.randn(10, 4, device=device, requires_grad=True)
+    node = ops.scaled_embedding(w, torch.arange(10, device=device)).grad_fn
+    ones = torch.ones(10, 4, device=device)
+    for bad in (ones.cpu(), ones.half(), ones.double(), ones.to_sparse()):
+        with pytest.raises(RuntimeError, match='must be a dense tensor'):
+            node(bad)
+    with pytest.raises(RuntimeError):
+        node(ones[:5])
+    assert torch.equal(node(ones)[0], ones)
+
+
 def test_two_streams_at_once(device):
     from tracevae_amd import ops
     g = torch.Generator().manual_seed(8)

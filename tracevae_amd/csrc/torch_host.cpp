@@ -11,10 +11,12 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <string>
+#include <unordered_set>
 #include <vector>
 
 #include "../../include/tracevae_hip.h"
@@ -57,6 +59,48 @@ void *stream_of(const at::Tensor &t) {
   return (void *)c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream();
 }
 
+bool capturing(const c10::Stream &s) {
+  const hipStream_t stream = c10::hip::HIPStreamMasqueradingAsCUDA(s).stream();
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (stream == nullptr) return false;            // (the default stream cannot be captured)
+  if (hipStreamIsCapturing(stream, &status) != hipSuccess) {
+    (void)hipGetLastError();
+    return false;
+  }
+  return status == hipStreamCaptureStatusActive;
+}
+
+// Autograd runs a node on the stream on which it was made and lets that stream wait for the node before it.
+// In a captured backward pass a node from outside the capture - the accumulator of a leaf that an eager
+// graph still holds - ties an eager stream to the capture, which ends the process: refused here, before
+// the engine gets there.
+void refuse_nodes_outside_capture(const c10::Stream &current) {
+  if (!capturing(current)) return;
+  const auto node = torch::autograd::get_current_node();
+  if (!node) return;
+  const auto *exec = torch::autograd::get_current_graph_task_exec_info();
+  std::vector<torch::autograd::Node *> todo{node.get()};
+  std::unordered_set<torch::autograd::Node *> seen;
+  while (!todo.empty()) {
+    torch::autograd::Node *at = todo.back();
+    todo.pop_back();
+    for (const auto &edge : at->next_edges()) {
+      torch::autograd::Node *next = edge.function.get();
+      if (!next || !seen.insert(next).second) continue;
+      if (exec && !exec->empty()) {               // (of autograd.grad: the nodes that it needs)
+        const auto it = exec->find(next);
+        if (it == exec->end() || !it->second.should_execute()) continue;
+      }
+      const auto stream = next->stream();
+      if (stream && *stream != current && !capturing(*stream))
+        throw LibraryError("scaled_embedding: this backward pass is being captured, but " + next->name() +
+                           " of a tensor it leads to belongs to an eager graph that is still alive: drop that "
+                           "graph's outputs before the capture");
+      todo.push_back(next);
+    }
+  }
+}
+
 // (behind the checks of scaled_embedding below: a [tokens, dim] table with contiguous rows, contiguous
 // int64 ids on its device, types that go together)
 at::Tensor lookup(const at::Tensor &weight, const at::Tensor &ids, double scale, int64_t padding_id, int64_t out_code) {
@@ -92,6 +136,14 @@ class ScaledEmbedding : public torch::autograd::Function<ScaledEmbedding> {
     const auto sizes = ctx->saved_data["sizes"].toIntVector();
     const int64_t tokens = sizes[0], dim = sizes[1], rows = ids.numel();
     const c10::DeviceGuard guard(ids.device());
+    // (autograd's engine hands over nothing else; a node that is called by hand may)
+    if (grads[0].device() != ids.device() || grads[0].layout() != at::kStrided ||
+        grads[0].scalar_type() != dtype_of(sizes[3]))
+      throw Mismatch(std::string("the gradient of the rows must be a dense tensor of their type (") +
+                     c10::toString(dtype_of(sizes[3])) + ") on " + ids.device().str() + ", got " +
+                     c10::toString(grads[0].scalar_type()) + " on " + grads[0].device().str());
+    refuse_nodes_outside_capture(
+        c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(ids.device().index()).unwrap());
     at::Tensor dw;
     {
       const at::AutoGradMode no_grad(false);
