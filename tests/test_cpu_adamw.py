@@ -66,6 +66,20 @@ def test_control_refuses():
     assert lib.tv_adamw_control(0, 1e-3, 0.9, 0.99, 1e-8, None) == -1
 
 
+def test_control_has_the_products_that_the_steps_form():
+    """beta^step as a product of `step` factors, bit for bit, while 1 - beta^step shows it."""
+    for step in (0, 1, 2, 37, 5000, 100000, 10 ** 12):
+        image = torch.zeros(hip.lib().tv_adamw_control_bytes() // 8, dtype=torch.int64)
+        assert hip.lib().tv_adamw_control(step, 1e-3, 0.9, 0.999, 1e-8, image.data_ptr()) == 0
+        got = image.view(torch.float64)[5:7].tolist()
+        want = [1.0, 1.0]
+        for _ in range(min(step, 100000)):
+            want = [want[0] * 0.9, want[1] * 0.999]
+        for x, y in zip(got, want):
+            assert x == y or (x <= 1e-30 and y <= 1e-30)
+        assert int(image[0]) == step
+
+
 def test_step_refuses_before_any_launch():
     lib = hip.lib()
     one = 1 << 20                       # never dereferenced: validation fails first

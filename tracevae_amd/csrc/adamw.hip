@@ -545,8 +545,18 @@ extern "C" int tv_adamw_control(int64_t step, double lr, double beta1, double be
   c.beta1 = beta1;
   c.beta2 = beta2;
   c.eps = eps;
-  c.beta1_t = pow(beta1, (double)step);
-  c.beta2_t = pow(beta2, (double)step);
+  // the product as the steps form it, so that a run that is taken up again has the same bits (what lies
+  // below 1e-30 no longer shows in 1 - beta^step); behind 2^24 steps, 20 ms, by pow
+  c.beta1_t = c.beta2_t = 1.0;
+  const int64_t factors = step < (1 << 24) ? step : 1 << 24;
+  for (int64_t t = 0; t < factors && (c.beta1_t > 1e-30 || c.beta2_t > 1e-30); ++t) {
+    c.beta1_t *= beta1;
+    c.beta2_t *= beta2;
+  }
+  if (step > factors) {
+    c.beta1_t *= pow(beta1, (double)(step - factors));
+    c.beta2_t *= pow(beta2, (double)(step - factors));
+  }
   *(Control *)control = c;
   return TV_OK;
 }
