@@ -246,7 +246,7 @@ struct Step {
   float keep, step_size, inv_sqrt_bc2, eps;       // keep = 1 - lr * weight_decay
   double coef, beta1, beta2, omb1, omb2;
   uint32_t key;
-  int it0, it1;                                   // which 1024 elements of the chunk
+  int it0, it1;                                   // which 4 * THREADS elements of the chunk
 };
 
 __device__ __forceinline__ float moved(float p, float m, float r, const Step &s) {
@@ -273,13 +273,13 @@ __device__ __forceinline__ float master_of(float p, float w) {
 template <>
 __device__ __forceinline__ float master_of<float>(float p, float) { return p; }
 
-template <typename T>
+template <int THREADS, typename T>
 __device__ __forceinline__ void chunk_step32(T *p, const T *g, float *w, float *m, float *v, int n,
                                              const Step &s) {
   const float b1 = (float)s.beta1, b2 = (float)s.beta2, o1 = (float)s.omb1, o2 = (float)s.omb2;
   const float coef = (float)s.coef;
   for (int it = s.it0; it < s.it1; ++it) {
-    const int i = it * 4 * AW_THREADS + (int)threadIdx.x * 4;
+    const int i = it * 4 * THREADS + (int)threadIdx.x * 4;
     if (i >= n) break;
     float px[4], gx[4], wx[4], mx[4], vx[4];
     load4(p, i, n, px);
@@ -371,13 +371,13 @@ __device__ __forceinline__ double inverse(float s) {
   return s > 0.f ? 1.0 / (double)s : 0.0;
 }
 
-template <typename T>
+template <int THREADS, typename T>
 __device__ __forceinline__ void chunk_step8(T *p, const T *g, float *w, uint32_t *m8, float *ms,
                                             uint32_t *r8, float *rs, int n, int64_t element0,
                                             const Step &s) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   for (int it = s.it0; it < s.it1; ++it) {
-    const int b = it * (4 * AW_THREADS / AW_BLOCK) + wave, i = b * AW_BLOCK + lane * 4;
+    const int b = it * (4 * THREADS / AW_BLOCK) + wave, i = b * AW_BLOCK + lane * 4;
     if (b * AW_BLOCK >= n) break;                 // (the same for the whole wave)
     // (blocks begin at multiples of 256: the high word is the same for the whole block)
     const uint32_t key = mix(s.key + (uint32_t)((element0 + b * AW_BLOCK) >> 32));
@@ -451,17 +451,18 @@ __device__ __forceinline__ void chunk_step8(T *p, const T *g, float *w, uint32_t
 
 // ALONE: without begin_kernel (no norm, no guard, few workgroups): every workgroup computes the scalars,
 // and the last one to finish - all others have read the counters by then - counts the step
-template <bool EIGHT, bool ALONE>
-__global__ __launch_bounds__(AW_THREADS) void adamw_step_kernel(
-    const void *plan, int64_t count, int64_t chunk0, int64_t tensor0, Grads grads, Control *ctl,
+template <bool EIGHT, bool ALONE, int THREADS>
+__global__ __launch_bounds__(THREADS) void adamw_step_kernel(
+    const void *plan, int64_t count, int64_t chunk0, int lg_parts, int64_t tensor0, Grads grads, Control *ctl,
     void *moment1, void *moment2, float *scale1, float *scale2, float *master, uint32_t seed_key) {
-  const Chunk ch = plan_chunks(plan, count)[chunk0 + blockIdx.x];
+  const Chunk ch = plan_chunks(plan, count)[chunk0 + (blockIdx.x >> lg_parts)];
   const void *g = grads.g[ch.tensor - tensor0];
   const int64_t base = (int64_t)ch.index * AW_CHUNK, at = ch.state;
   const int n = ch.n;
   Step s;
-  s.it0 = blockIdx.y * (AW_ITS / gridDim.y);
-  s.it1 = s.it0 + AW_ITS / gridDim.y;
+  const int part = (int)blockIdx.x & ((1 << lg_parts) - 1), its = AW_CHUNK / (4 * THREADS) >> lg_parts;
+  s.it0 = part * its;
+  s.it1 = s.it0 + its;
   s.keep = (float)(1.0 - ctl->lr * ch.weight_decay);
   s.beta1 = ctl->beta1;
   s.beta2 = ctl->beta2;
@@ -487,26 +488,26 @@ __global__ __launch_bounds__(AW_THREADS) void adamw_step_kernel(
   }
   // (tested behind the loads above, which are in flight together.  Without a gradient the tensor stays
   // as it is)
-  if (!skip && g != nullptr && s.it0 * (4 * AW_THREADS) < n) {
+  if (!skip && g != nullptr && s.it0 * (4 * THREADS) < n) {
     float *w = master ? master + at : nullptr;
     if (EIGHT) {
       s.key = mix(seed_key + (uint32_t)step);
       uint32_t *m8 = (uint32_t *)moment1 + at / 4, *r8 = (uint32_t *)moment2 + at / 4;
       float *ms = scale1 + at / AW_BLOCK, *rs = scale2 + at / AW_BLOCK;
       if (ch.dtype == TV_DTYPE_F32)
-        chunk_step8((float *)ch.param, (const float *)g + base, w, m8, ms, r8, rs, n, at, s);
+        chunk_step8<THREADS>((float *)ch.param, (const float *)g + base, w, m8, ms, r8, rs, n, at, s);
       else if (ch.dtype == TV_DTYPE_BF16)
-        chunk_step8((__bf16 *)ch.param, (const __bf16 *)g + base, w, m8, ms, r8, rs, n, at, s);
+        chunk_step8<THREADS>((__bf16 *)ch.param, (const __bf16 *)g + base, w, m8, ms, r8, rs, n, at, s);
       else
-        chunk_step8((_Float16 *)ch.param, (const _Float16 *)g + base, w, m8, ms, r8, rs, n, at, s);
+        chunk_step8<THREADS>((_Float16 *)ch.param, (const _Float16 *)g + base, w, m8, ms, r8, rs, n, at, s);
     } else {
       float *m = (float *)moment1 + at, *v = (float *)moment2 + at;
       if (ch.dtype == TV_DTYPE_F32)
-        chunk_step32((float *)ch.param, (const float *)g + base, w, m, v, n, s);
+        chunk_step32<THREADS>((float *)ch.param, (const float *)g + base, w, m, v, n, s);
       else if (ch.dtype == TV_DTYPE_BF16)
-        chunk_step32((__bf16 *)ch.param, (const __bf16 *)g + base, w, m, v, n, s);
+        chunk_step32<THREADS>((__bf16 *)ch.param, (const __bf16 *)g + base, w, m, v, n, s);
       else
-        chunk_step32((_Float16 *)ch.param, (const _Float16 *)g + base, w, m, v, n, s);
+        chunk_step32<THREADS>((_Float16 *)ch.param, (const _Float16 *)g + base, w, m, v, n, s);
     }
   }
   if (ALONE) {
@@ -515,7 +516,7 @@ __global__ __launch_bounds__(AW_THREADS) void adamw_step_kernel(
     // this workgroup has written is read in this launch (and such a fence writes the L2 back: 2 us).
     __syncthreads();
     if (threadIdx.x == 0 && __hip_atomic_fetch_add(&ctl->ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
-                                gridDim.x * gridDim.y - 1) {
+                                gridDim.x - 1) {
       ctl->ticket = 0;
       ctl->step = step;
       ctl->beta1_t = b1t;
@@ -680,10 +681,6 @@ extern "C" int tv_adamw_step(const void *plan_host, const void *plan_device,
     chunk0 = tensors[t0].first_chunk;
     chunk1 = t1 < plan->count ? tensors[t1].first_chunk : plan->chunks;
   };
-  // Workgroups per chunk.  Few chunks: 4, each a quarter of the latency (62 000 parameters, 32 bits: 4.3
-  // us against 6.0; 2.3 million, 8 bits: 13.8 against 16.8).  Many: 2 with 32-bit moments (343 million:
-  // 1.83 ms against 1.87), 1 with 8-bit ones, whose scalars per workgroup weigh more (1.10 against 1.11).
-  const unsigned parts = plan->chunks <= 1024 ? 4 : state_bits == 32 ? 2 : 1;
   int64_t nblk = 0;
   double *partial = (double *)workspace;
   for (int64_t k = 0; clip_norm > 0.0 && k < ngroups; ++k) {
@@ -708,17 +705,26 @@ extern "C" int tv_adamw_step(const void *plan_host, const void *plan_device,
                        norm_out, guard, guard_kind, guard_copy);
     TV_LAUNCH_CHECK("tv_adamw_step");
   }
+  // A chunk is the work of 2^lg workgroups side by side.  Many small ones, which begin and end one by one,
+  // stream best: with 32-bit moments 268 million fp32 parameters take 1190 us in 8 x 128 threads, 1258 in
+  // 4 x 256, 1276 in 1 x 1024 (bf16: 1332, 1336, 1384).  The scalars of a workgroup weigh more with 8-bit moments:
+  // 729 us in 4 x 128, 797 in 8 x 128 - up to 256 chunks the other way round, 9.9 against 9.1.  The one-
+  // launch step takes fewer tickets with 2 x 512: 64 chunks 5.5-6.6 us against 6.5-7.1 in 4 x 256.
+  const int lg = alone ? 1 : state_bits == 32 || plan->chunks <= 256 ? 3 : 2;
+  constexpr int64_t launch_chunks = 1 << 21;      // (a launch has less than 2^32 threads)
   for (int64_t k = 0; k < ngroups; ++k) {
     Grads g = {};
     int64_t c0, c1;
     group_grads(k, g, c0, c1);
-    if (c1 == c0) continue;
-    auto kernel = state_bits == 8 ? (alone ? adamw_step_kernel<true, true> : adamw_step_kernel<true, false>)
-                                  : (alone ? adamw_step_kernel<false, true> : adamw_step_kernel<false, false>);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(c1 - c0), parts), dim3(AW_THREADS), 0, (hipStream_t)stream,
-                       plan_device, plan->count, c0, k * AW_GRADS, g, (Control *)control,
-                       moment1, moment2, scale1, scale2, master, mix((uint32_t)seed));
-    TV_LAUNCH_CHECK("tv_adamw_step");
+    for (int64_t c = c0; c < c1; c += launch_chunks) {
+      auto kernel = state_bits == 8 ? (alone ? adamw_step_kernel<true, true, 512> : adamw_step_kernel<true, false, 128>)
+                                    : (alone ? adamw_step_kernel<false, true, 512> : adamw_step_kernel<false, false, 128>);
+      const int64_t n = c1 - c < launch_chunks ? c1 - c : launch_chunks;
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(n << lg)), dim3(alone ? 512 : 128), 0, (hipStream_t)stream, plan_device,
+                         plan->count, c, lg, k * AW_GRADS, g, (Control *)control, moment1, moment2, scale1, scale2,
+                         master, mix((uint32_t)seed));
+      TV_LAUNCH_CHECK("tv_adamw_step");
+    }
   }
   return TV_OK;
 }
