@@ -87,19 +87,19 @@ template <typename T> struct Four {                // four elements, at any alig
   typedef T V __attribute__((ext_vector_type(4)));
   typedef V Any __attribute__((aligned(sizeof(T))));
 };
-// four consecutive elements from i on, zeros behind n
-template <typename T>
-__device__ __forceinline__ void load4(const T *p, int i, int n, float (&x)[4]) {
+// Four consecutive elements from i on, zeros behind n.  They are widened apart from the load: a conversion
+// in the branch would wait for the load there, and the next one would start behind it.
+template <typename T> __device__ __forceinline__ typename Four<T>::V load4(const T *p, int i, int n) {
   const AW_GLOBAL T *q = (const AW_GLOBAL T *)(p + i);
-  if (i + 4 <= n) {
-    typedef typename Four<T>::Any Any;
-    const typename Four<T>::V f = __builtin_nontemporal_load((const AW_GLOBAL Any *)q);
+  if (i + 4 <= n) return __builtin_nontemporal_load((const AW_GLOBAL typename Four<T>::Any *)q);
+  typename Four<T>::V x;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = (float)f[j];
-  } else {
+  for (int j = 0; j < 4; ++j) x[j] = i + j < n ? q[j] : (T)0.f;
+  return x;
+}
+template <typename V> __device__ __forceinline__ void widen(V f, float (&x)[4]) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = i + j < n ? (float)q[j] : 0.f;
-  }
+  for (int j = 0; j < 4; ++j) x[j] = (float)f[j];
 }
 template <typename T>
 __device__ __forceinline__ void store4(T *p, int i, int n, const float (&x)[4]) {
@@ -282,11 +282,12 @@ __device__ __forceinline__ void chunk_step32(T *p, const T *g, float *w, float *
     const int i = it * 4 * THREADS + (int)threadIdx.x * 4;
     if (i >= n) break;
     float px[4], gx[4], wx[4], mx[4], vx[4];
-    load4(p, i, n, px);
-    load4(g, i, n, gx);
+    const auto p4 = load4(p, i, n), g4 = load4(g, i, n);
     load4(m, i, mx);
     load4(v, i, vx);
     if (sizeof(T) != 4) load4(w, i, wx);
+    widen(p4, px);
+    widen(g4, gx);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float gj = gx[j] * coef;
@@ -383,12 +384,14 @@ __device__ __forceinline__ void chunk_step8(T *p, const T *g, float *w, uint32_t
     const uint32_t key = mix(s.key + (uint32_t)((element0 + b * AW_BLOCK) >> 32));
     const uint32_t element = (uint32_t)(element0 + i);
     float px[4], gx[4], wx[4], mo[4], ro[4];
-    load4(p, i, n, px);
-    load4(g, i, n, gx);
-    decode4(__builtin_nontemporal_load(m8 + i / 4), mo);
-    decode4(__builtin_nontemporal_load(r8 + i / 4), ro);
+    const auto p4 = load4(p, i, n), g4 = load4(g, i, n);
+    const uint32_t m4 = __builtin_nontemporal_load(m8 + i / 4), r4 = __builtin_nontemporal_load(r8 + i / 4);
     if (sizeof(T) != 4) load4(w, i, wx);
     const double sm = ms[b], sr = rs[b];
+    widen(p4, px);
+    widen(g4, gx);
+    decode4(m4, mo);
+    decode4(r4, ro);
     const double k2 = s.beta2 * (sr * sr);
     double mx[4], rx[4];
     uint32_t am = 0, ar = 0;                      // bits of the largest |m| and rms in fp32
@@ -707,10 +710,15 @@ extern "C" int tv_adamw_step(const void *plan_host, const void *plan_device,
   }
   // A chunk is the work of 2^lg workgroups side by side.  Many small ones, which begin and end one by one,
   // stream best: with 32-bit moments 268 million fp32 parameters take 1190 us in 8 x 128 threads, 1258 in
-  // 4 x 256, 1276 in 1 x 1024 (bf16: 1332, 1336, 1384).  The scalars of a workgroup weigh more with 8-bit moments:
-  // 729 us in 4 x 128, 797 in 8 x 128 - up to 256 chunks the other way round, 9.9 against 9.1.  The one-
-  // launch step takes fewer tickets with 2 x 512: 64 chunks 5.5-6.6 us against 6.5-7.1 in 4 x 256.
+  // 4 x 256, 1276 in 1 x 1024 (bf16: 1332, 1336, 1384).  The scalars of a workgroup weigh more with 8-bit
+  // moments: 729 us in 4 x 128, 797 in 8 x 128 - up to 256 chunks the other way round, 9.9 against 9.1.
+  // The one-launch step takes fewer tickets with 2 x 512: 64 chunks 5.5-6.6 us against 6.5-7.1 in 4 x 256.
   const int lg = alone ? 1 : state_bits == 32 || plan->chunks <= 256 ? 3 : 2;
+  // Large models, 32 bits: 24 KB of LDS that nobody uses leave 6 such workgroups on a CU, which reads and writes
+  // memory in longer runs: 537 million fp32 2401 us against 2507, bf16 2569 against 2733; 25 million 113.1
+  // against 113.9 and 121 against 124, 14 million with clipping 81.4 against 77.4.  (Not for 8-bit moments, which
+  // need the waves to cover their arithmetic: 878 against 723.)
+  const unsigned lds = state_bits == 32 && plan->chunks > 4096 ? 24 << 10 : 0;
   constexpr int64_t launch_chunks = 1 << 21;      // (a launch has less than 2^32 threads)
   for (int64_t k = 0; k < ngroups; ++k) {
     Grads g = {};
@@ -720,7 +728,7 @@ extern "C" int tv_adamw_step(const void *plan_host, const void *plan_device,
       auto kernel = state_bits == 8 ? (alone ? adamw_step_kernel<true, true, 512> : adamw_step_kernel<true, false, 128>)
                                     : (alone ? adamw_step_kernel<false, true, 512> : adamw_step_kernel<false, false, 128>);
       const int64_t n = c1 - c < launch_chunks ? c1 - c : launch_chunks;
-      hipLaunchKernelGGL(kernel, dim3((unsigned)(n << lg)), dim3(alone ? 512 : 128), 0, (hipStream_t)stream, plan_device,
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(n << lg)), dim3(alone ? 512 : 128), lds, (hipStream_t)stream, plan_device,
                          plan->count, c, lg, k * AW_GRADS, g, (Control *)control, moment1, moment2, scale1, scale2,
                          master, mix((uint32_t)seed));
       TV_LAUNCH_CHECK("tv_adamw_step");
