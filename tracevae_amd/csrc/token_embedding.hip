@@ -22,6 +22,7 @@
 namespace {
 
 constexpr int TE_THREADS = 256;
+constexpr int TE_LOOKUP_THREADS = 512;
 constexpr int TE_SORT_THREADS = 1024;             // of a sort workgroup
 constexpr int TE_SORT_WAVES = TE_SORT_THREADS / 64;
 constexpr int TE_TINY = 128;                      // rows whose gradient is one launch
@@ -83,16 +84,17 @@ __device__ __forceinline__ int64_t part_column(int64_t part, int n, int64_t dim)
 // stored past the caches: a lookup of 64, 256 and 512 MiB takes 20, 77 and 153 us so and 21, 85 and 178
 // without the hint, a lookup and one pass that reads its result 42, 177 and 343 against 41, 181 and 355 -
 // and without it what follows pays for the dirty lines (lookup and gradient of 32768 x 1024: 101 us
-// against 113).
+// against 113).  512 threads and 2 rows each: 65536 x 4096 bf16 135 us (256 and 4: 143, 512 and 1: 173, 1024
+// and 2: 142), 16384 x 4096 fp32 68 (83, 76, 65), 262144 x 512 bf16 40 (44, 73, 42).
 // ---------------------------------------------------------------------------------------
 template <typename W, typename O, int N, int ROWS>
-__global__ __launch_bounds__(TE_THREADS) void lookup_kernel(int64_t rows, int64_t dim, int64_t vocab,
+__global__ __launch_bounds__(TE_LOOKUP_THREADS) void lookup_kernel(int64_t rows, int64_t dim, int64_t vocab,
                                                             int parts, int lg, const W *__restrict__ weight,
                                                             int64_t weight_stride,
                                                             const int64_t *__restrict__ ids,
                                                             int64_t padding, float scale,
                                                             O *__restrict__ out, int64_t out_stride) {
-  const int per = TE_THREADS >> lg;               // rows per workgroup and trip
+  const int per = TE_LOOKUP_THREADS >> lg;               // rows per workgroup and trip
   const int64_t r0 = (int64_t)blockIdx.x * per * ROWS + (threadIdx.x >> lg);
   int64_t id[ROWS];
 #pragma unroll
@@ -657,12 +659,13 @@ void launch_lookup_n(int64_t rows, int64_t dim, int64_t vocab, const void *weigh
                      hipStream_t stream) {
   const int parts = (int)tv_cdiv(dim, N);
   int lg = 0;
-  while ((1 << lg) < parts && lg < 8) ++lg;
-  const int64_t per = TE_THREADS >> lg;
-  // four rows per thread where that leaves four workgroups per CU
-  const bool four = tv_cdiv(rows, per) >= 4096;
-  auto kernel = four ? lookup_kernel<W, O, N, 4> : lookup_kernel<W, O, N, 1>;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)tv_cdiv(rows, per * (four ? 4 : 1))), dim3(TE_THREADS), 0, stream, rows,
+  while ((1 << lg) < parts && lg < 9) ++lg;
+  const int64_t per = TE_LOOKUP_THREADS >> lg;
+  // two rows per thread where that leaves two workgroups per CU (4096 x 1024 bf16 3.4 us against 3.9 with one,
+  // 2048 x 1024 2.85 against 2.79)
+  const bool two = tv_cdiv(rows, per) >= 1024;
+  auto kernel = two ? lookup_kernel<W, O, N, 2> : lookup_kernel<W, O, N, 1>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)tv_cdiv(rows, per * (two ? 2 : 1))), dim3(TE_LOOKUP_THREADS), 0, stream, rows,
                      dim, vocab, parts, lg, (const W *)weight, weight_stride, ids, padding, scale, (O *)out,
                      out_stride);
 }
