@@ -325,16 +325,16 @@ __global__ __launch_bounds__(TE_SORT_THREADS) void digit_scatter_kernel(
 // ---------------------------------------------------------------------------------------
 // sums over the sorted list
 // ---------------------------------------------------------------------------------------
-// Rows of dW that no token names, 16 per wave: a binary search in the sorted list for each.  They are
-// stored past the caches (50001 x 1024 fp32, three quarters of it zeros: 102 us for lookup and gradient
-// against 110 without; the rows that hold sums lose by it, 118).
+// Rows of dW that no token names, `each` (up to 16) per wave: a binary search in the sorted list for each.
+// They are stored past the caches (50001 x 1024 fp32, three quarters of it zeros: 102 us for lookup and
+// gradient against 110 without; the rows that hold sums lose by it, 118).
 template <typename W>
-__device__ __forceinline__ void zero_absent_rows(int64_t wave, int64_t n, int64_t dim, int64_t vocab,
+__device__ __forceinline__ void zero_absent_rows(int64_t wave, int each, int64_t n, int64_t dim, int64_t vocab,
                                                  const uint2 *__restrict__ sorted, W *__restrict__ dweight) {
   const int lane = threadIdx.x & 63;
-  const int64_t v0 = wave * 16, v = v0 + lane;
+  const int64_t v0 = wave * each, v = v0 + lane;
   bool absent = false;
-  if (lane < 16 && v < vocab) {
+  if (lane < each && v < vocab) {
     int64_t lo = 0, hi = n;                       // the first pair whose token is not below v
     while (lo < hi) {
       const int64_t mid = (lo + hi) >> 1;
@@ -369,11 +369,11 @@ __device__ __forceinline__ void zero_absent_rows(int64_t wave, int64_t n, int64_
 template <typename D, typename W, int N, int G>
 __global__ __launch_bounds__(TE_THREADS) void tile_sums_kernel(
     int64_t n, int64_t dim, int64_t vocab, int tile, int64_t tiles, int64_t slabs, int64_t tile_blocks,
-    const uint2 *__restrict__ sorted, const D *__restrict__ dout, int64_t dout_stride, float scale,
+    int zero_rows, const uint2 *__restrict__ sorted, const D *__restrict__ dout, int64_t dout_stride, float scale,
     W *__restrict__ dweight, float *__restrict__ part) {
   if ((int64_t)blockIdx.x >= tile_blocks) {
-    zero_absent_rows<W>(((int64_t)blockIdx.x - tile_blocks) * (TE_THREADS / 64) + (threadIdx.x >> 6), n, dim,
-                        vocab, sorted, dweight);
+    zero_absent_rows<W>(((int64_t)blockIdx.x - tile_blocks) * (TE_THREADS / 64) + (threadIdx.x >> 6), zero_rows, n,
+                        dim, vocab, sorted, dweight);
     return;
   }
   const int64_t unit = (int64_t)blockIdx.x * (TE_THREADS / G) + threadIdx.x / G;
@@ -707,9 +707,16 @@ void launch_sums_ng(const Shape &s, int64_t rows, int64_t dim, int64_t vocab, co
                     const void *dout, int64_t dout_stride, float scale, void *dweight, float *part,
                     hipStream_t stream) {
   const int64_t slabs = tv_cdiv(tv_cdiv(dim, N), G), units = s.tiles * slabs;
-  const int64_t tile_blocks = tv_cdiv(units, TE_THREADS / G), zero_blocks = tv_cdiv(vocab, 16 * (TE_THREADS / 64));
+  // Rows of zeros per wave: the wider they are the fewer, so that memory is written from end to end by waves that
+  // come and go.  Gradient of 32768 x 1024 into 50001 fp32 rows of 4 KB with 16, 8, 4 per wave: 85, 81, 79 us,
+  // of 16384 x 1024 into 200001: 181, 168, 179; of 8192 x 4096 into 50001 bf16 rows of 8 KB: 123, 119, 111; of
+  // 131072 x 256 into 100001 fp32 rows of 1 KB: 83, 85, 97.
+  const int64_t bytes = dim * (int64_t)sizeof(W);
+  const int zero_rows = vocab > (1 << 24) || bytes <= 1024 ? 16 : bytes <= 4096 ? 8 : 4;
+  const int64_t tile_blocks = tv_cdiv(units, TE_THREADS / G);
+  const int64_t zero_blocks = tv_cdiv(vocab, zero_rows * (TE_THREADS / 64));
   hipLaunchKernelGGL((tile_sums_kernel<D, W, N, G>), dim3((unsigned)(tile_blocks + zero_blocks)), dim3(TE_THREADS),
-                     0, stream, rows, dim, vocab, (int)s.tile, s.tiles, slabs, tile_blocks, sorted,
+                     0, stream, rows, dim, vocab, (int)s.tile, s.tiles, slabs, tile_blocks, zero_rows, sorted,
                      (const D *)dout, dout_stride, scale, (W *)dweight, part);
   if (s.tiles > 1)
     hipLaunchKernelGGL((join_kernel<W, N, G>), dim3((unsigned)tv_cdiv(units, TE_JOIN_THREADS / G)),
