@@ -226,6 +226,22 @@ def test_more_than_2_to_the_31_elements(device):
     torch.cuda.empty_cache()
 
 
+def test_a_lookup_of_more_rows_than_one_launch_takes(device):
+    """2^23 + 5 rows of 1028 fp32 (34.5 GB): one workgroup for every two rows, 2^22 in a launch."""
+    from tracevae_amd import ops
+    if torch.cuda.mem_get_info()[0] < 48 << 30:
+        pytest.skip('needs 48 GiB of free GPU memory')
+    rows, dim, v = 2 ** 23 + 5, 1028, 1000
+    w = torch.randn(v, dim, device=device)
+    ids = torch.arange(rows, device=device) * 7 % v
+    out = ops.scaled_embedding(w, ids, 1.0)
+    for r0 in (0, rows // 2, 2 ** 23 - 1000, rows - 1000):
+        assert torch.equal(out[r0:r0 + 1000], w[ids[r0:r0 + 1000]])
+    assert torch.equal(out[:, 5], w[:, 5][ids]) and torch.equal(out[:, -1], w[:, -1][ids])
+    del out
+    torch.cuda.empty_cache()
+
+
 def test_captured_and_replayed(device):
     """Forward and gradient in one captured graph, replayed on new ids with eager calls of another size
     between the replays: equal to the eager result every time."""

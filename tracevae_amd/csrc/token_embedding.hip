@@ -94,7 +94,7 @@ __global__ __launch_bounds__(TE_LOOKUP_THREADS) void lookup_kernel(int64_t rows,
                                                             const int64_t *__restrict__ ids,
                                                             int64_t padding, float scale,
                                                             O *__restrict__ out, int64_t out_stride) {
-  const int per = TE_LOOKUP_THREADS >> lg;               // rows per workgroup and trip
+  const int per = TE_LOOKUP_THREADS >> lg;        // rows per workgroup and trip
   const int64_t r0 = (int64_t)blockIdx.x * per * ROWS + (threadIdx.x >> lg);
   int64_t id[ROWS];
 #pragma unroll
@@ -665,9 +665,13 @@ void launch_lookup_n(int64_t rows, int64_t dim, int64_t vocab, const void *weigh
   // 2048 x 1024 2.85 against 2.79)
   const bool two = tv_cdiv(rows, per) >= 1024;
   auto kernel = two ? lookup_kernel<W, O, N, 2> : lookup_kernel<W, O, N, 1>;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)tv_cdiv(rows, per * (two ? 2 : 1))), dim3(TE_LOOKUP_THREADS), 0, stream, rows,
-                     dim, vocab, parts, lg, (const W *)weight, weight_stride, ids, padding, scale, (O *)out,
-                     out_stride);
+  const int64_t each = per * (two ? 2 : 1), most = each << 22;      // (a launch has less than 2^32 threads)
+  for (int64_t r = 0; r < rows; r += most) {
+    const int64_t n = rows - r < most ? rows - r : most;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)tv_cdiv(n, each)), dim3(TE_LOOKUP_THREADS), 0, stream, n, dim, vocab, parts,
+                       lg, (const W *)weight, weight_stride, ids + r, padding, scale, (O *)out + r * out_stride,
+                       out_stride);
+  }
 }
 template <typename W, typename O>
 void launch_lookup(int64_t rows, int64_t dim, int64_t vocab, const void *weight, int64_t weight_stride,
