@@ -479,13 +479,14 @@ __global__ __launch_bounds__(TE_JOIN_THREADS) void join_kernel(int64_t n, int64_
     const uint32_t cur = sorted[i1 - 1].x;
     const uint32_t next = sorted[i1].x, head = sorted[i0].x, prev = sorted[i0 > 0 ? i0 - 1 : 0].x;
     if (cur < vocab && next == cur && !(head == cur && i0 > 0 && prev == cur)) {
-      int64_t lo = t + 1, hi = tiles;             // the first tile that does not begin with the token
-      // (the next G tiles at once: a token seldom has more)
-      const int64_t probe = t + 1 + lane;
-      const bool in = probe < tiles && sorted[probe * tile].x == cur;
-      const uint64_t all = __ballot(in);
-      const uint64_t mine = (G == 64 ? all : (all >> ((threadIdx.x & 63) & ~(G - 1)))) & (G == 64 ? ~0ull : ((1ull << (G & 63)) - 1ull));
-      const int run = __popcll(mine);
+      // the first tile that does not begin with the token, by G probes at a time: first the next G tiles
+      // (a token seldom has more), then G of the rest
+      auto run_of = [&](int64_t probe, int64_t end) -> int {
+        const uint64_t all = __ballot(probe < end && sorted[(probe < end ? probe : end - 1) * tile].x == cur);
+        return __popcll(G == 64 ? all : (all >> ((threadIdx.x & 63) & ~(G - 1))) & ((1ull << (G & 63)) - 1ull));
+      };
+      int64_t lo = t + 1, hi = tiles;
+      const int run = run_of(lo + lane, hi);
       if (run < G && run <= TE_LONG) {
         float acc[N];
         load_n<N, float>(part + (t * 2 + 1) * dim + col, acc);
@@ -494,12 +495,11 @@ __global__ __launch_bounds__(TE_JOIN_THREADS) void join_kernel(int64_t n, int64_
         for (int j = 0; j < N; ++j) acc[j] *= scale;
         if (active) store_n<N, W>(dweight + (int64_t)cur * dim + col, acc);
       } else {
-        lo = t + 1 + run;
-        if (run < G) hi = lo;
-        while (lo < hi) {
-          const int64_t mid = (lo + hi) >> 1;
-          if (sorted[mid * tile].x == cur) lo = mid + 1;
-          else hi = mid;
+        lo += run;
+        while (run == G && lo < hi) {
+          const int64_t step = (hi - lo + G - 1) / G;
+          lo += run_of(lo + (lane + 1) * step - 1, hi) * step;
+          hi = lo + step - 1 < hi ? lo + step - 1 : hi;
         }
         if (lane == 0) long_end[group] = lo;
       }
