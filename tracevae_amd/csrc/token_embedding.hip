@@ -437,7 +437,9 @@ __global__ __launch_bounds__(TE_THREADS) void tile_sums_kernel(
 
 // The token that begins in tile t and goes on behind it: its slot there, then slot 0 of the tiles
 // that follow, in order.  A group of G lanes takes the token of one tile; one of more than TE_LONG
-// tiles is left to the whole workgroup, whose groups take one run of its tiles each.
+// tiles is left to the whole workgroup, whose groups take one run of its tiles each.  The slabs of a token
+// are in different workgroups (32768 x 2048 fp32 over 1000 tokens 70 us against 86 with the slabs side by
+// side, 65536 x 4096 bf16 over 32000 168 against 189): one CU reads no more than some 100 GB/s.
 template <typename W, int N, int G>
 __global__ __launch_bounds__(TE_JOIN_THREADS) void join_kernel(int64_t n, int64_t dim, int64_t vocab, int tile,
                                                                int64_t tiles, int64_t slabs,
@@ -450,8 +452,9 @@ __global__ __launch_bounds__(TE_JOIN_THREADS) void join_kernel(int64_t n, int64_
   const int group = threadIdx.x / G, lane = threadIdx.x % G;
   auto tile_of = [&](int g, int64_t &t, int64_t &col) -> bool {
     const int64_t unit = (int64_t)blockIdx.x * GROUPS + g;
-    t = unit / slabs;
-    const int64_t column_part = (unit - t * slabs) * G + lane;
+    const int64_t slab = unit / tiles;
+    t = slab < slabs ? unit - slab * tiles : tiles;
+    const int64_t column_part = slab * G + lane;
     const bool active = column_part * N < dim;
     col = active ? part_column(column_part, N, dim) : 0;
     return active;
