@@ -633,12 +633,12 @@ inline Shape shape_of(int64_t rows, int64_t dim, int64_t vocab) {
   // one run of ids per sort workgroup
   s.items = tv_cdiv(tv_cdiv(rows, TE_SORT_BLOCKS), TE_SORT_THREADS) * TE_SORT_THREADS;
   s.nblk = (int)tv_cdiv(rows, s.items > 0 ? s.items : 1);
-  // Rows per tile: the longest that leaves 1024 waves (four per CU), between 8 and 128.  Longer tiles
-  // leave fewer sums to join, shorter ones more rows in flight: 32768 rows of 1024 bf16 in tiles of 16,
-  // 64 and 128 take 55 + 17, 58 + 12 and 74 + 8 us (tiles + join), 1021 rows of 251 fp16 in tiles of 8 and
-  // 32 take 5.2 + 5.2 and 11.8 + 4.3, 262144 of 512 bf16 in 64 and 128 take 83 + 22 and 83 + 16.
+  // Rows per tile: the longest that leaves 2048 waves (eight per CU), between 8 and 128.  Longer tiles leave
+  // fewer sums to join, shorter ones more rows in flight: 32768 rows of 1024 bf16 into 50001 fp32 take 104, 79,
+  // 72 and 74 us with tiles that leave 512, 1024, 2048 and 4096 waves, 262144 of 64 bf16 86, 69, 65 and 66;
+  // 262144 of 512 bf16 in tiles of 128 take 76 us, of 256 87.
   s.tile = 8;
-  while (s.tile < 128 && rows * slots / (s.tile * 2) >= 1024 * 64) s.tile *= 2;
+  while (s.tile < 128 && rows * slots / (s.tile * 2) >= 2048 * 64) s.tile *= 2;
   s.tiles = tv_cdiv(rows, s.tile);
   const bool small = rows <= TE_SMALL;
   s.pairs0 = 0;
