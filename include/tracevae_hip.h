@@ -47,7 +47,7 @@ extern "C" {
 #define TV_DTYPE_F32 0
 #define TV_DTYPE_BF16 1
 #define TV_DTYPE_F16 2
-/* tv_adamw_*: elements that share the scale of their 8-bit moments, elements per workgroup */
+/* tv_adamw_*: elements that share the scale of their 8-bit moments, elements per chunk of the plan */
 #define TV_ADAMW_BLOCK 256
 #define TV_ADAMW_CHUNK 4096
 

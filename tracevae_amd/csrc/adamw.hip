@@ -6,13 +6,13 @@
 //   p  = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
 // The tensors stay where they are: a plan in device memory lists them and cuts each one into chunks
-// of 4096 elements, one workgroup per chunk; the gradients' addresses, which autograd changes from
-// step to step, travel as kernel arguments.  Everything is elementwise and bound by HBM: 28 bytes
+// of 4096 elements, the work of a few small workgroups; the gradients' addresses, which autograd changes
+// from step to step, travel as kernel arguments.  Everything is elementwise and bound by HBM: 28 bytes
 // per fp32 parameter with 32-bit moments, 16.06 with 8-bit ones, 30 / 18.06 per 16-bit one with its
 // master, and the gradient once more for the norm.  Measured (kernels alone): 343 million bf16
-// parameters, 32 bits: 1.83 ms, 10.3 GB at 5.6 TB/s, norm 0.11 ms; fp32, 8 bits: 0.98 ms, 5.5 GB at 5.6
-// TB/s; 14 million in 152 tensors: 62 us + 12 + 3 for the norm, 8 bits 46 + 12 + 3; 62 000 in 16
-// tensors: 3.4 us.
+// parameters, 32 bits: 1.59 ms, 10.3 GB at 6.5 TB/s, norm 0.11 ms; fp32, 8 bits: 0.93 ms, 5.5 GB at 5.9
+// TB/s; 14 million in 152 tensors: 60 us + 14 + 5 for the norm, 8 bits 41 + 14 + 4; 62 000 in 16
+// tensors: 4.3 us.
 //
 // 8-bit moments: m / s_m and sqrt(v) / s_r in e4m3 with s = max over the block / 448, so that the
 // largest element sits on the largest code.  The codes are rounded STOCHASTICALLY, from a hash of
@@ -31,7 +31,7 @@
 namespace {
 
 constexpr int AW_THREADS = 256;
-constexpr int AW_CHUNK = TV_ADAMW_CHUNK;          // elements per workgroup
+constexpr int AW_CHUNK = TV_ADAMW_CHUNK;
 constexpr int AW_BLOCK = TV_ADAMW_BLOCK;          // elements per scale: one wave, 4 per lane
 constexpr int AW_ITS = AW_CHUNK / (4 * AW_THREADS);
 constexpr int AW_GRADS = 384;                     // gradient addresses per launch (3 KB of arguments)
@@ -77,9 +77,8 @@ __host__ __device__ inline const Chunk *plan_chunks(const void *plan, int64_t co
 
 // Every access carries the hint that nothing of it is read again soon: between two steps a forward and
 // a backward pass go through the caches.  Alternating between three models, with the hint against
-// without: 14 million parameters 82 us against 95 (32 bits), 60 against 68 (8 bits), 343 million
-// 1.96 ms against 2.11 and 1.01 against 1.06.  (One model stepped over and over, whose 228 MB stay in
-// the 256 MB last-level cache, takes 64 us with it and 60 without.)
+// without: 14 million parameters 78 us against 89 (32 bits), 57 against 65 (8 bits), 343 million
+// 1.70 ms against 1.98 and 0.94 against 1.03.
 // Parameters and gradients come by addresses out of memory, which the compiler takes for generic ones
 // (flat accesses, which wait for LDS as well): they are global.
 #define AW_GLOBAL __attribute__((address_space(1)))
@@ -725,12 +724,12 @@ extern "C" int tv_adamw_step(const void *plan_host, const void *plan_device,
     int64_t c0, c1;
     group_grads(k, g, c0, c1);
     for (int64_t c = c0; c < c1; c += launch_chunks) {
-      auto kernel = state_bits == 8 ? (alone ? adamw_step_kernel<true, true, 512> : adamw_step_kernel<true, false, 128>)
-                                    : (alone ? adamw_step_kernel<false, true, 512> : adamw_step_kernel<false, false, 128>);
+      auto kernel = alone ? (state_bits == 8 ? adamw_step_kernel<true, true, 512> : adamw_step_kernel<false, true, 512>)
+                          : (state_bits == 8 ? adamw_step_kernel<true, false, 128> : adamw_step_kernel<false, false, 128>);
       const int64_t n = c1 - c < launch_chunks ? c1 - c : launch_chunks;
-      hipLaunchKernelGGL(kernel, dim3((unsigned)(n << lg)), dim3(alone ? 512 : 128), lds, (hipStream_t)stream, plan_device,
-                         plan->count, c, lg, k * AW_GRADS, g, (Control *)control, moment1, moment2, scale1, scale2,
-                         master, mix((uint32_t)seed));
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(n << lg)), dim3(alone ? 512 : 128), lds, (hipStream_t)stream,
+                         plan_device, plan->count, c, lg, k * AW_GRADS, g, (Control *)control, moment1, moment2,
+                         scale1, scale2, master, mix((uint32_t)seed));
       TV_LAUNCH_CHECK("tv_adamw_step");
     }
   }

@@ -12,11 +12,11 @@
 // token that crosses tile borders go to a workspace and are joined in tile order.  Sums are fp32, in
 // a fixed order, rounded once; no atomics on floats, so results repeat bit for bit.
 //
-// Measured (kernels alone): lookup of 65536 x 4096 bf16 117 us (835 MB read and written,
-// 7.1 TB/s).  Gradient of 262144 x 512 bf16 over 1000 tokens, half of the rows on three of
+// Measured (kernels alone): lookup of 65536 x 4096 bf16 116 us (837 MB read and written,
+// 7.2 TB/s).  Gradient of 262144 x 512 bf16 over 1000 tokens, half of the rows on three of
 // them: sort 5 + 13, tiles 49 (268 MB read, 5.5 TB/s), join 15 us.  Of 32768 x 1024 bf16 into 50001 fp32
-// rows: sort 17, tiles and zero rows 45 (268 MB, 5.9 TB/s), join 10.  Of 25600 x 40 fp32 over 1000: sort 3
-// + 7, tiles 5, join 13; of 1021 x 251 fp16: sort 6, tiles 5, join 5 - a chain of dependent loads each.
+// rows: sort 18, tiles and zero rows 46 (269 MB, 5.8 TB/s), join 9.  Of 25600 x 40 fp32 over 1000: sort 3
+// + 7, tiles 6, join 13; of 1021 x 251 fp16: sort 6, tiles 6, join 6 - a chain of dependent loads each.
 #include "tv_common.h"
 
 namespace {
@@ -81,10 +81,10 @@ __device__ __forceinline__ int64_t part_column(int64_t part, int n, int64_t dim)
 
 // ---------------------------------------------------------------------------------------
 // Forward: 2^lg threads per row, ROWS rows per thread with their loads in flight together.  The rows are
-// stored past the caches: a lookup of 64, 256 and 512 MiB takes 20, 77 and 153 us so and 21, 85 and 178
-// without the hint, a lookup and one pass that reads its result 42, 177 and 343 against 41, 181 and 355 -
-// and without it what follows pays for the dirty lines (lookup and gradient of 32768 x 1024: 101 us
-// against 113).  512 threads and 2 rows each: 65536 x 4096 bf16 135 us (256 and 4: 143, 512 and 1: 173, 1024
+// stored past the caches: a lookup of 64, 256 and 512 MiB takes 17, 62 and 133 us so and 18, 75 and 144
+// without the hint, a lookup and one pass that reads its result 37, 132 and 252 against 35, 138 and 271 -
+// and without it what follows pays for the dirty lines (lookup and gradient of 32768 x 1024: 92 us
+// against 107).  512 threads and 2 rows each: 65536 x 4096 bf16 135 us (256 and 4: 143, 512 and 1: 173, 1024
 // and 2: 142), 16384 x 4096 fp32 68 (83, 76, 65), 262144 x 512 bf16 40 (44, 73, 42).
 // ---------------------------------------------------------------------------------------
 template <typename W, typename O, int N, int ROWS>
@@ -326,8 +326,8 @@ __global__ __launch_bounds__(TE_SORT_THREADS) void digit_scatter_kernel(
 // sums over the sorted list
 // ---------------------------------------------------------------------------------------
 // Rows of dW that no token names, `each` (up to 16) per wave: a binary search in the sorted list for each.
-// They are stored past the caches (50001 x 1024 fp32, three quarters of it zeros: 102 us for lookup and
-// gradient against 110 without; the rows that hold sums lose by it, 118).
+// They are stored past the caches (50001 x 1024 fp32, three quarters of it zeros: 92 us for lookup and
+// gradient against 101 without; the rows that hold sums lose by it).
 template <typename W>
 __device__ __forceinline__ void zero_absent_rows(int64_t wave, int each, int64_t n, int64_t dim, int64_t vocab,
                                                  const uint2 *__restrict__ sorted, W *__restrict__ dweight) {
@@ -671,9 +671,9 @@ void launch_lookup_n(int64_t rows, int64_t dim, int64_t vocab, const void *weigh
   const int64_t each = per * (two ? 2 : 1), most = each << 22;      // (a launch has less than 2^32 threads)
   for (int64_t r = 0; r < rows; r += most) {
     const int64_t n = rows - r < most ? rows - r : most;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)tv_cdiv(n, each)), dim3(TE_LOOKUP_THREADS), 0, stream, n, dim, vocab, parts,
-                       lg, (const W *)weight, weight_stride, ids + r, padding, scale, (O *)out + r * out_stride,
-                       out_stride);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)tv_cdiv(n, each)), dim3(TE_LOOKUP_THREADS), 0, stream, n, dim, vocab,
+                       parts, lg, (const W *)weight, weight_stride, ids + r, padding, scale,
+                       (O *)out + r * out_stride, out_stride);
   }
 }
 template <typename W, typename O>
