@@ -462,6 +462,43 @@ def test_elements_beyond_32_bits(device):
     torch.cuda.empty_cache()
 
 
+def test_more_chunks_than_one_launch_takes(device):
+    """2^33 + 5000 elements (8-bit moments): the elements on both sides of the second launch's beginning."""
+    from tracevae_amd.optim import AdamW
+    if torch.cuda.mem_get_info()[0] < 112 << 30:
+        pytest.skip('needs 112 GiB of free GPU memory')
+    n, a, b = 2 ** 33 + 5000, 2 ** 33 - 1024, 2 ** 33 + 1024
+    p = torch.zeros(n, device=device)
+    g = torch.zeros(n, device=device)
+    gen = torch.Generator().manual_seed(4)
+    p[a:b] = torch.randn(b - a, generator=gen).to(device)
+    g[a:b] = torch.randn(b - a, generator=gen).to(device)
+    p[-1] = g[-1] = 1.0
+    p0, g0 = p[a:b].cpu().double(), g[a:b].cpu().double()
+    opt = AdamW([p], weight_decay=0.1, state_bits=8, seed=5, **HYPER)
+    opt.step([g])
+    p1, m1, v1, change = ref.step(p0, g0, 0.0, torch.zeros(b - a).double(), 1, 1e-2, 0.9, 0.999, 1e-8, 0.1, 1.0)
+    assert ((p[a:b].cpu().double() - p1).abs() <= 3 * U * (p0.abs() + change.abs()) + 8 * U * change.abs()).all()
+    words = ref.random_words(torch.arange(a, b), 5, 1).view(-1, 256)
+    q, scale = ref.to_codes((1 - 0.9) * g0.view(-1, 256), words & 0xffff, False)
+    assert torch.equal(opt.state['exp_avg8'][a:b].cpu().double(), q.view(-1))
+    assert float(p[-1]) < 1.0 and opt.steps == 1
+    del p, g, opt
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_a_large_model_with_32_bit_moments(device, dtype):
+    """More than 4096 chunks, where fewer workgroups share a CU, with and without clipping."""
+    from tracevae_amd.optim import AdamW
+    shapes = [(300,), (4096 * 4096 + 777,), (3, 5)]
+    params = _params(shapes, dtype, device, 51)
+    opt = AdamW(params, weight_decay=0.1, **HYPER)
+    twin = Twin(opt, [0.1] * 3)
+    for k, clip in enumerate((1.0, None)):
+        twin.step(_grads(params, 52 + k), clip)
+
+
 def test_refusals(device):
     from tracevae_amd import hip
     from tracevae_amd.optim import AdamW
