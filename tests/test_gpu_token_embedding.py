@@ -102,6 +102,19 @@ def test_long_batches(device, rows, vocab, dim, kind):
     _check(w.bfloat16(), ids, 0.5, None, torch.bfloat16, torch.randn(rows, dim, generator=g).bfloat16(), device)
 
 
+@pytest.mark.parametrize('rows,vocab,dim', [(700, 1501, 513), (700, 1499, 1030), (5000, 401, 2051), (3000, 33, 1280)])
+@pytest.mark.parametrize('kind', ['zipf', 'same', 'runs'])
+def test_wide_rows(device, rows, vocab, dim, kind):
+    """Absent rows of 1 to 8 KB, tokens of many tiles in several slabs of columns."""
+    g = torch.Generator().manual_seed(rows + vocab + dim)
+    ids = _ids(kind, rows, vocab, g)
+    w = torch.randn(vocab, dim, generator=g)
+    d = torch.randn(rows, dim, generator=g)
+    for table, out_dtype in ((torch.float32, torch.float32), (torch.float32, torch.bfloat16),
+                             (torch.float16, torch.float16)):
+        _check(w.to(table), ids, 0.5, vocab // 2, out_dtype, d.to(out_dtype), device)
+
+
 def test_no_rows_and_nothing_but_padding(device):
     for table, out_dtype in TYPES:
         w = torch.randn(70, 24).to(table)
