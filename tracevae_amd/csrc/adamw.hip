@@ -698,9 +698,9 @@ extern "C" int tv_adamw_step(const void *plan_host, const void *plan_device,
     nblk += blocks;
   }
   // One launch where nothing has to be known before it and few workgroups take a ticket: the tickets are
-  // taken one after another, 12 ns each.  A step of 64 chunks (256 workgroups) 6.1-6.8 us against 7.1-8.6
-  // with the launch of the scalars, of 128 chunks 9.2-9.9 against 7.1-8.7, of 1024 chunks 52 against 19-26.
-  const bool alone = clip_norm == 0.0 && !guard && ngroups == 1 && plan->chunks > 0 && plan->chunks <= 64;
+  // taken one after another, 12 ns each.  A step of 64 chunks 4.9-6.3 us against 8.7-8.9 with the launch of
+  // the scalars, of 128 chunks 7.3-7.7 against 8.6-9.0, of 192 chunks the same, of 512 chunks 17 against 12-15.
+  const bool alone = clip_norm == 0.0 && !guard && ngroups == 1 && plan->chunks > 0 && plan->chunks <= 128;
   if (!alone) {
     hipLaunchKernelGGL(adamw_begin_kernel, dim3(1), dim3(clip_norm > 0.0 ? AW_BEGIN_THREADS : 64), 0,
                        (hipStream_t)stream, (Control *)control, clip_norm > 0.0, nblk, partial, clip_norm,
