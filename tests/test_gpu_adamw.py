@@ -387,6 +387,37 @@ def test_a_moved_parameter_is_found(device):
         assert torch.equal(params[0], twins[0])
 
 
+@pytest.mark.parametrize('bits', [32, 8])
+def test_the_plan_of_a_captured_step_outlives_a_move(device, bits):
+    """An eager step over a parameter that has moved makes a new plan; a captured one goes on with the plan that
+    it was captured with, over the tensor that was there."""
+    import weakref
+    from tracevae_amd.optim import AdamW
+    params = _params(ODD, torch.float32, device, 81)
+    opt = AdamW(params, state_bits=bits, **HYPER)
+    g = _grads(params, 82)
+    opt.step(g)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step(g)
+    plan, image = weakref.ref(opt._plan), opt._plan.clone()
+    first = params[0].data
+    for _ in range(3):
+        params[0].set_(params[0].clone())
+        opt.step(g)
+        junk = [torch.full_like(image, -1) for _ in range(4)]       # takes what was freed
+    assert plan() is not None and torch.equal(plan(), image)
+    assert opt._plan is not plan() and all(x.data_ptr() != plan().data_ptr() for x in junk)
+    for k in range(2):
+        here, there = params[0].clone(), first.clone()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(params[0], here) and not torch.equal(first, there)
+        assert opt.steps == 5 + k
+    assert torch.isfinite(first).all() and len(opt._captured_plans) == 1
+
+
 def test_on_a_stream_of_its_own(device):
     from tracevae_amd.optim import AdamW
     params = _params([(100000,)], torch.float32, device, 26)

@@ -36,8 +36,9 @@ class AdamW(object):
     * all state buffers are flat: tensor i begins at `offsets[i]`, a multiple of 256.
     * the step counter and the learning rate are on the device: `step()` never waits for the GPU and
       may be captured into a graph (capture after the first eager step; `set_lr` between replays is
-      seen by them).  A tensor whose gradient is None is left as it is, state included; the step
-      counter is one for all tensors.
+      seen by them).  A replay updates the parameters where they were when it was captured, and needs
+      the optimizer to be alive.  A tensor whose gradient is None is left as it is, state included; the
+      step counter is one for all tensors.
     * calls on one optimizer must be ordered: one stream, or events between them.
     """
 
@@ -100,6 +101,7 @@ class AdamW(object):
         self._workspace = zeros(int(lib.tv_adamw_workspace_bytes(n)) // 8, torch.float64)
         self.grad_norm = torch.zeros((), dtype=torch.float64, device=self.device)
         self._plan = None
+        self._captured_plans = []                 # read by every replay of the steps captured with them
         self._make_plan()
 
     # -- set-up ------------------------------------------------------------------------
@@ -197,6 +199,9 @@ class AdamW(object):
         clip = float(global_clip_norm or 0.0)
         if grads is not None and type(grads) is not list:
             grads = list(grads)
+        capturing = torch.cuda.is_current_stream_capturing()
+        if capturing and not any(p is self._plan for p in self._captured_plans):
+            self._captured_plans.append(self._plan)
         step = hip.host().adamw_step
         while not step(self.params, grads, *self._fixed, clip,
                        self.grad_norm.data_ptr() if clip else None, self.seed, hip.ptr(guard),
@@ -205,7 +210,7 @@ class AdamW(object):
                        self._workspace.data_ptr(), self._workspace.numel() * 8, hip.stream(),
                        self.device.index):
             # a parameter is not where it was
-            if torch.cuda.is_current_stream_capturing():
+            if capturing:
                 raise hip.HipLibraryError('a parameter has moved since the last step: take one '
                                           'eager step before capturing')
             self._make_plan()
