@@ -214,6 +214,49 @@ def test_no_second_derivative_and_no_changed_ids(device):
     assert not ops.scaled_embedding(w.detach(), ids, 2.0).requires_grad
 
 
+@pytest.mark.parametrize('requires', [False, True])
+@pytest.mark.parametrize('grad', [False, True])
+def test_a_tangent_of_the_table_is_refused(device, requires, grad):
+    import torch.autograd.forward_ad as forward
+    from tracevae_amd import ops
+    ids = torch.arange(60, device=device) % 30
+    w = torch.randn(30, 8, device=device).requires_grad_(requires)
+    with forward.dual_level(), torch.set_grad_enabled(grad):
+        dual = forward.make_dual(w, torch.ones_like(w))
+        with pytest.raises(NotImplementedError, match='forward'):
+            ops.scaled_embedding(dual, ids, 2.0)
+
+
+def test_a_tangent_of_the_gradient_is_refused(device):
+    import torch.autograd.forward_ad as forward
+    from tracevae_amd import ops
+    w = torch.randn(30, 8, device=device, requires_grad=True)
+    out = ops.scaled_embedding(w, torch.arange(60, device=device) % 30, 2.0)
+    ones = torch.ones(60, 8, device=device)
+    with forward.dual_level():
+        with pytest.raises(NotImplementedError, match='forward'):
+            torch.autograd.grad(out, w, forward.make_dual(ones, ones))
+
+
+def test_function_transforms_are_refused(device):
+    from tracevae_amd import ops
+    w = torch.randn(30, 8, device=device)
+    ids = torch.arange(60, device=device) % 30
+
+    def look(x):
+        return ops.scaled_embedding(x, ids, 2.0)
+
+    for call in (lambda: torch.func.vmap(lambda i: ops.scaled_embedding(w, i))(ids.view(2, 30)),
+                 lambda: torch.func.vmap(look)(torch.stack([w, w])),
+                 lambda: torch.func.grad(lambda x: look(x).sum())(w),
+                 lambda: torch.func.jvp(look, (w,), (w,))):
+        with pytest.raises(RuntimeError):
+            call()
+    x = w.clone().requires_grad_(True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(look(x), x, torch.ones(2, 60, 8, device=device), is_grads_batched=True)
+
+
 def test_more_than_2_to_the_31_elements(device):
     """bf16 rows of 2^21 + 5 tokens by 1030 columns: positions beyond 32 bits in the rows and in their
     gradient (4.3 GB each)."""

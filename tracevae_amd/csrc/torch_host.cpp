@@ -101,6 +101,12 @@ void refuse_nodes_outside_capture(const c10::Stream &current) {
   }
 }
 
+// A lookup hands on no tangent: a result without one would read as a derivative of zero.
+void refuse_tangent(const at::Tensor &t, const char *what) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), "scaled_embedding: ", what,
+                              " carries a tangent, forward mode is not implemented");
+}
+
 // (behind the checks of scaled_embedding below: a [tokens, dim] table with contiguous rows, contiguous
 // int64 ids on its device, types that go together)
 at::Tensor lookup(const at::Tensor &weight, const at::Tensor &ids, double scale, int64_t padding_id, int64_t out_code) {
@@ -142,6 +148,7 @@ class ScaledEmbedding : public torch::autograd::Function<ScaledEmbedding> {
       throw Mismatch(std::string("the gradient of the rows must be a dense tensor of their type (") +
                      c10::toString(dtype_of(sizes[3])) + ") on " + ids.device().str() + ", got " +
                      c10::toString(grads[0].scalar_type()) + " on " + grads[0].device().str());
+    refuse_tangent(grads[0], "the gradient of the rows");
     refuse_nodes_outside_capture(
         c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(ids.device().index()).unwrap());
     at::Tensor dw;
@@ -207,6 +214,8 @@ template <typename F> PyObject *guarded(F f) {
     PyErr_SetString(PyExc_ValueError, e.what());
   } catch (const python_error &) {
     // (set already)
+  } catch (const c10::NotImplementedError &e) {
+    PyErr_SetString(PyExc_NotImplementedError, e.what_without_backtrace());
   } catch (const c10::OutOfMemoryError &e) {
     PyErr_SetString(memory_error, e.what());
   } catch (const std::exception &e) {
@@ -239,6 +248,7 @@ PyObject *scaled_embedding(PyObject *, PyObject *const *args, Py_ssize_t n) {
       throw Mismatch(std::string("ids must be torch.int64, got ") + c10::toString(ids.scalar_type()));
     if (weight.layout() != at::kStrided || ids.layout() != at::kStrided) throw Mismatch("weight and ids are dense");
     if (weight.dim() != 2 || weight.numel() == 0) throw std::invalid_argument("weight must be [tokens, dim]");
+    refuse_tangent(weight, "weight");
     at::Tensor out;
     {
       struct Released {                           // (also when an exception passes)
