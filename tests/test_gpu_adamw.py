@@ -667,3 +667,69 @@ def test_trainer_runs_both_phases_with_adamw(device, kind):
     with torch.no_grad():
         bad.copy_(keep)
     assert torch.equal(before, trainer.flat.flat) and trainer.optimizer.adamw.steps == steps
+
+
+def _trainer(flags):
+    from helpers import make_config, make_flat
+    from tracevae_amd.batch import DeviceTraceStore, TraceGraphBatch
+    from tracevae_amd.config import parse_flags
+    from tracevae_amd.model import TraceVAE
+    from tracevae_amd.train import Trainer
+    flat, lr = make_flat(16, 30, 12)
+    cfg = make_config()
+    parse_flags(cfg, flags)
+    torch.manual_seed(0)
+    vae = TraceVAE(cfg.model, 30, max_node_count=12).to('cuda')
+    trainer = Trainer(vae, cfg, world_size=1)
+    return trainer, TraceGraphBatch.from_store(DeviceTraceStore(flat, lr, 30), np.arange(16), 12)
+
+
+@pytest.mark.parametrize('latency_only', [False, True])
+@pytest.mark.parametrize('kind', ['adamw', 'adamw8'])
+def test_trainer_decays_in_place_of_the_l2_term(device, kind, latency_only):
+    """Loss and gradients are those of a model without the L2 term, and one update is AdamW's on them: clipped
+    to 10, biases not decayed."""
+    a, G = _trainer([f'--train.optimizer={kind}'])
+    b, _ = _trainer(['--train.l2_reg=0'])
+    got = []
+    for trainer in (a, b):
+        trainer.set_phase(latency_only)
+        torch.manual_seed(1)
+        got.append(trainer.local_gradients(G)['loss'].detach())
+    assert torch.equal(got[0], got[1])
+    start = a.optimizer.start
+    assert torch.equal(a.flat.grad[start:], b.flat.grad[start:])
+    assert torch.equal(a.flat.flat, b.flat.flat)
+    grad, before = a.flat.grad.cpu().double(), a.flat.flat.cpu().double()
+    a.update()
+    used = torch.zeros_like(grad)
+    decay = torch.zeros_like(grad)
+    for n in a.flat.names:
+        at, end = a.flat.slices[n][0], a.flat.slices[n][0] + a.flat.params[n].numel()
+        if at >= start:
+            used[at:end] = 1
+            decay[at:end] = 0.0 if 'bias' in n else 0.01
+    coef = min(1.0, 10.0 / (float((grad * used).square().sum().sqrt()) + 1e-6))
+    p1, m1, v1, change = ref.step(before, grad, torch.zeros_like(grad), torch.zeros_like(grad), 1, a.optimizer.lr,
+                                  0.9, 0.999, 1e-8, decay, coef)
+    # the bound at the top, with M = |m| in a first step, and the steps of 2^-149 as in Twin.step
+    size = a.optimizer.lr / (1 - 0.9) / (v1.sqrt() / math.sqrt(1 - 0.999) + 1e-8)
+    bound = 3 * U * (before.abs() + change.abs()) + 16 * U * change.abs() + 2.0 ** -149 * (size + a.optimizer.lr * 10 + 1)
+    after = a.flat.flat.cpu().double()
+    assert ((after - p1).abs() <= bound)[used > 0].all()
+    assert torch.equal(after[used == 0], before[used == 0])
+    assert float(change[used > 0].abs().max()) > 0
+
+
+def test_trainer_refuses_a_regulariser_that_its_optimizer_does_not_use(device):
+    from tracevae_amd.train import FlatOptimizer
+    for flags, name in ((['--train.optimizer=adamw', '--train.l2_reg=0.001'], 'l2_reg'),
+                        (['--train.optimizer=adam', '--train.weight_decay=0.1'], 'weight_decay'),
+                        (['--train.weight_decay=0.1'], 'weight_decay')):
+        with pytest.raises(ValueError, match=f'does not use train.{name}'):
+            _trainer(flags)
+    trainer, _ = _trainer(['--train.weight_decay=0', '--train.l2_reg=0.001'])
+    assert trainer.l2_reg == 0.001
+    with pytest.raises(ValueError, match='no weight decay'):
+        FlatOptimizer(trainer.flat, 'adam', weight_decay=0.1)
+    assert _trainer(['--train.optimizer=adamw8', '--train.l2_reg=0'])[0].l2_reg is None

@@ -181,14 +181,14 @@ class ExpConfig(Config):
         val_epoch_freq: Optional[int] = 2
         kl_beta = 1.0
         warm_up_epochs: Optional[int] = None
-        l2_reg = 0.0001
+        l2_reg = 0.0001          # of 'rmsprop' / 'adam'
         z_unit_ball_reg: Optional[float] = None
         z2_unit_ball_reg: Optional[float] = None
         init_batch_size = 64
         batch_size = 64
         val_batch_size = 64
         optimizer = 'rmsprop'    # 'adam' | 'rmsprop'; not in the reference: 'adamw' | 'adamw8'
-        weight_decay = 0.01      # of 'adamw' / 'adamw8' (biases are left out)
+        weight_decay = 0.01      # of 'adamw' / 'adamw8', in place of l2_reg (biases are left out)
         initial_lr = 0.001
         lr_anneal_ratio = 0.1
         lr_anneal_epochs = 30

@@ -6,7 +6,8 @@ Restates `tracegnn/models/trace_vae/train.py`:
 * two-phase schedule (all parameters, then `latency_vae.*` only with the rest
   of the model in eval mode), LR annealing from the global epoch                :204-208, 374-383, 455-487
 * clip by global norm 10 + RMSprop / Adam (tensorkit `fit_model`)               :369-372, 417-426
-  (beyond the reference: AdamW, `--train.optimizer=adamw` / `adamw8`)
+  (beyond the reference: AdamW, `--train.optimizer=adamw` / `adamw8`, whose decoupled weight decay
+  stands in the place of the L2 term in the loss)
 * `models/{epoch}.pt`, `models/final.pt` = `torch.save(vae.state_dict())`        :343-352
 
 MI355X-side design: all parameters live in ONE flat fp32 buffer (struct part first, the
@@ -143,6 +144,9 @@ class FlatParameters(object):
             torch._foreach_copy_(dst, src)
 
 
+DECOUPLED = ('adamw', 'adamw8')        # optimizers that decay the weights themselves
+
+
 class FlatOptimizer(object):
     """RMSprop / Adam over a range of the flat buffer, with clip-by-global-norm
     (`tv_sumsq_partial` -> `tv_sum_partials` -> `tv_optim_step`); or AdamW over the parameters of
@@ -153,10 +157,10 @@ class FlatOptimizer(object):
                  end: Optional[int] = None, alpha: float = 0.99, betas=(0.9, 0.999),
                  eps: float = 1e-8, weight_decay: float = 0.0, seed: int = 0):
         self.flat, self.kind = flat, kind.lower()
-        if self.kind not in ('rmsprop', 'adam', 'adamw', 'adamw8'):
+        if self.kind not in ('rmsprop', 'adam') + DECOUPLED:
             raise ValueError(f'unknown optimizer {kind!r}')
         self.start, self.end = start, flat.total if end is None else end
-        if self.kind in ('adamw', 'adamw8'):
+        if self.kind in DECOUPLED:
             names = [n for n in flat.names if self.start <= flat.slices[n][0] < self.end]
             self._grads = [flat.grad_views[n] for n in names]
             self.adamw = AdamW([flat.params[n].data for n in names], betas=betas, eps=eps,
@@ -165,6 +169,8 @@ class FlatOptimizer(object):
             self.lr = self.adamw.lr
             self.grad_norm = self.adamw.grad_norm
             return
+        if weight_decay:
+            raise ValueError(f'{kind!r} takes no weight decay')
         self.adamw = None
         n = self.end - self.start
         dev = flat.flat.device
@@ -275,8 +281,15 @@ class Trainer(object):
         for n, p in f.params.items():
             p.requires_grad_(n in in_part)
         start = f.tail_start if latency_only else 0
-        self.optimizer = FlatOptimizer(f, self.train_cfg.optimizer, start, f.total,
-                                       weight_decay=self.train_cfg.weight_decay,
+        kind = self.train_cfg.optimizer
+        decoupled = kind.lower() in DECOUPLED
+        unused = 'l2_reg' if decoupled else 'weight_decay'
+        value = getattr(self.train_cfg, unused)
+        if value and value != getattr(ExpConfig.train, unused):
+            raise ValueError(f'train.optimizer={kind} does not use train.{unused} (={value}): rmsprop and adam take '
+                             f'l2_reg, an L2 term in the loss; adamw and adamw8 take weight_decay')
+        self.optimizer = FlatOptimizer(f, kind, start, f.total,
+                                       weight_decay=self.train_cfg.weight_decay if decoupled else 0.0,
                                        seed=self.config.seed or 0)
         self.optimizer.set_lr(learning_rate_for_epoch(self.train_cfg, self.epoch - 1))
         self.l2_names = l2_parameter_names(f.all_names, part)
@@ -302,6 +315,12 @@ class Trainer(object):
         self.optimizer.set_lr(learning_rate_for_epoch(self.train_cfg, epoch - 1))
 
     # -- one step ----------------------------------------------------------------------
+    @property
+    def l2_reg(self) -> Optional[float]:
+        """The weight of the L2 term in loss and gradients; none beside decoupled weight decay, which it would
+        put into the moments and the clipped norm a second time."""
+        return None if self.optimizer.adamw is not None else self.train_cfg.l2_reg
+
     def l2_value(self) -> torch.Tensor:
         f = self.flat
         hip.call('tv_sumsq_partial', f.total, hip.ptr(f.flat), hip.ptr(self.l2_mask),
@@ -312,7 +331,7 @@ class Trainer(object):
 
     def forward_loss(self, G: TraceGraphBatch, eps=None) -> Dict[str, torch.Tensor]:
         chain = self.vae.q(G, eps=eps).chain(self.vae.p, G=G)
-        l2 = self.l2_value() if self.train_cfg.l2_reg else None
+        l2 = self.l2_value() if self.l2_reg else None
         out = compute_train_loss(chain, self.train_cfg, l2, self.epoch)
         out['chain'] = chain
         return out
@@ -325,9 +344,9 @@ class Trainer(object):
         out = self.forward_loss(G, eps)
         out['loss'].backward()
         f.collect_grads()
-        if self.train_cfg.l2_reg:
+        if self.l2_reg:
             # d(l2_reg * sum p^2)/dp = 2 * l2_reg * p on the masked elements
-            hip.call('tv_axpy_masked', f.total, 2.0 * self.train_cfg.l2_reg, hip.ptr(f.flat),
+            hip.call('tv_axpy_masked', f.total, 2.0 * self.l2_reg, hip.ptr(f.flat),
                      hip.ptr(self.l2_mask), hip.ptr(f.grad))
         return out
 
