@@ -358,6 +358,46 @@ def test_state_dict_continues_bit_for_bit(device):
             assert torch.equal(opt.state[k].view(torch.uint8), again.state[k].view(torch.uint8))
 
 
+@pytest.mark.parametrize('bits', [32, 8])
+@pytest.mark.parametrize('how', ['deepcopy', 'save'])
+def test_a_copy_of_an_optimizer_stands_alone(device, bits, how):
+    """The copy has parameters, state and addresses of its own: it steps on when the original is gone, and
+    leaves the original as it was."""
+    import gc
+    import io
+    from tracevae_amd.optim import AdamW
+    params = _params(ODD, torch.bfloat16, device, 85)
+    opt = AdamW(params, weight_decay=0.1, state_bits=bits, seed=3, **HYPER)
+    opt.step(_grads(params, 86), 1.0)
+    opt.set_lr(5e-3)
+    if how == 'deepcopy':
+        twin = copy.deepcopy(opt)
+    else:                                         # (plain pickle does not take torch's 8-bit tensors back)
+        file = io.BytesIO()
+        torch.save(opt, file)
+        file.seek(0)
+        twin = torch.load(file, weights_only=False)
+    at = {x.data_ptr() for x in [*params, *opt.state.values(), opt._plan, opt.grad_norm] if x.numel()}
+    mine = [x for x in [*twin.params, *twin.state.values(), twin._plan, twin.grad_norm] if x.numel()]
+    assert not at & {x.data_ptr() for x in mine}
+    kept = [x.clone() for x in [*params, *opt.state.values()]]
+    twin.step(_grads(params, 87))
+    for a, b in zip([*params, *opt.state.values()], kept):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    assert opt.steps == 1 and twin.steps == 2
+    for k, clip in enumerate((None, 1.0, None)):
+        opt.step(_grads(params, 87 + k), clip)
+    want = [x.clone() for x in [*params, *opt.state.values()]]
+    del opt, params, kept
+    gc.collect()
+    for k, clip in ((1, 1.0), (2, None)):
+        twin.set_lr(5e-3)
+        twin.step(_grads(twin.params, 87 + k), clip)
+    for a, b in zip([*twin.params, *twin.state.values()], want):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    assert twin.steps == 4
+
+
 def test_the_master_follows_a_weight_that_was_written(device):
     from tracevae_amd.optim import AdamW
     for bits in (32, 8):

@@ -69,10 +69,8 @@ class AdamW(object):
                 raise ValueError(f'parameter {i} must be contiguous')
         self.state_bits, self.seed = state_bits, int(seed)
         self.betas, self.eps, self.lr = (float(betas[0]), float(betas[1])), float(eps), float(lr)
-        self._sizes = hip.array_type(ctypes.c_int64, n)(*[p.numel() for p in self.params])
-        self._dtypes = hip.array_type(ctypes.c_int, n)(*[_DTYPES[p.dtype] for p in self.params])
-        self._decay = hip.array_type(ctypes.c_double, n)(*decay)
-        self._addresses = hip.array_type(ctypes.c_int64, n)()
+        self.weight_decay = decay
+        self._make_arrays()
         lib = hip.lib()
         total = int(lib.tv_adamw_state_elements(n, self._sizes))
         self.offsets, at = [], 0
@@ -96,15 +94,37 @@ class AdamW(object):
             for at, p in zip(self.offsets, self.params):
                 self._state['master'][at:at + p.numel()].copy_(p.detach().reshape(-1))
         self._control = zeros(int(lib.tv_adamw_control_bytes()) // 8, torch.int64)
-        self._lr = self._control.view(torch.float64)[1]
         self._write_control(0)
         self._workspace = zeros(int(lib.tv_adamw_workspace_bytes(n)) // 8, torch.float64)
         self.grad_norm = torch.zeros((), dtype=torch.float64, device=self.device)
+        self._start()
+
+    # -- set-up ------------------------------------------------------------------------
+    def _make_arrays(self) -> None:
+        n = len(self.params)
+        self._sizes = hip.array_type(ctypes.c_int64, n)(*[p.numel() for p in self.params])
+        self._dtypes = hip.array_type(ctypes.c_int, n)(*[_DTYPES[p.dtype] for p in self.params])
+        self._decay = hip.array_type(ctypes.c_double, n)(*self.weight_decay)
+        self._addresses = hip.array_type(ctypes.c_int64, n)()
+
+    def _start(self) -> None:
+        self._lr = self._control.view(torch.float64)[1]
         self._plan = None
         self._captured_plans = []                 # read by every replay of the steps captured with them
         self._make_plan()
 
-    # -- set-up ------------------------------------------------------------------------
+    # a copy has addresses of its own: those of its arrays, buffers and parameters, not the original's
+    _ADDRESSED = ('_sizes', '_dtypes', '_decay', '_addresses', '_where', '_plan', '_plan_host', '_captured_plans',
+                  '_fixed', '_lr')
+
+    def __getstate__(self):
+        return {k: v for k, v in self.__dict__.items() if k not in self._ADDRESSED}
+
+    def __setstate__(self, state) -> None:
+        self.__dict__.update(state)
+        self._make_arrays()
+        self._start()
+
     def _call_host(self, name: str, *args) -> None:
         if getattr(hip.lib(), name)(*args) != 0:
             msg = hip.lib().tv_last_error().decode('utf-8', 'replace')
