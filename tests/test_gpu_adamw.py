@@ -196,6 +196,24 @@ def test_tensors_without_gradient_and_strided_gradients(device, bits):
 
 
 @pytest.mark.parametrize('bits', [32, 8])
+def test_gradients_with_the_sign_pending(device, bits):
+    from tracevae_amd.optim import AdamW
+    params = _params([(300,), (1,)], torch.float32, device, 61)
+    opt = AdamW(params, weight_decay=0.01, state_bits=bits, **HYPER)
+    twin = Twin(opt, [0.01] * 2)
+    g = _grads(params, 62)
+    given = [torch._neg_view(-g[0]), torch.complex(torch.zeros_like(g[1]), -g[1]).conj().imag]
+    assert all(x.is_neg() for x in given)
+    twin.step(g, 1.0, given)
+    with pytest.raises(ValueError):
+        AdamW([torch._neg_view(torch.ones(5, device=device))])
+    params[0].data = torch._neg_view(torch.ones(300, device=device))
+    if params[0].is_neg():
+        with pytest.raises(TypeError):
+            opt.step(g)
+
+
+@pytest.mark.parametrize('bits', [32, 8])
 def test_more_tensors_than_one_launch_takes(device, bits):
     from tracevae_amd.optim import AdamW
     shapes = [(1 + (i * 37) % 300,) for i in range(900)] + [(5000,)]

@@ -257,6 +257,22 @@ def test_function_transforms_are_refused(device):
         torch.autograd.grad(look(x), x, torch.ones(2, 60, 8, device=device), is_grads_batched=True)
 
 
+@pytest.mark.parametrize('dim', [1, 6])
+def test_views_with_the_opposite_sign(device, dim):
+    """The imaginary part of a conjugate is a view of the values with the sign pending."""
+    from tracevae_amd import ops
+    w = torch.randn(30, dim, device=device)
+    ids = torch.arange(60, device=device) % 30
+    assert torch.equal(ops.scaled_embedding(torch._neg_view(w), ids, 2.0), -2 * w[ids])
+    x = w.clone().requires_grad_(True)
+    d = torch.randn(60, dim, dtype=torch.complex64, device=device)
+    (want,) = torch.autograd.grad(ops.scaled_embedding(x, ids, 2.0), x, -d.imag.clone())
+    for dout in (d.conj().imag, torch._neg_view(d.imag.contiguous())):
+        assert dout.is_neg()
+        (dw,) = torch.autograd.grad(ops.scaled_embedding(x, ids, 2.0), x, dout)
+        assert torch.equal(dw, want)
+
+
 def test_more_than_2_to_the_31_elements(device):
     """bf16 rows of 2^21 + 5 tokens by 1030 columns: positions beyond 32 bits in the rows and in their
     gradient (4.3 GB each)."""

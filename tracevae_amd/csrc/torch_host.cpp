@@ -154,7 +154,7 @@ class ScaledEmbedding : public torch::autograd::Function<ScaledEmbedding> {
     at::Tensor dw;
     {
       const at::AutoGradMode no_grad(false);
-      at::Tensor dout = grads[0].reshape({rows, dim});
+      at::Tensor dout = grads[0].resolve_neg().reshape({rows, dim});
       const bool rows_apart = rows <= 1 || dout.stride(0) >= dim, dense_rows = dim <= 1 || dout.stride(1) == 1;
       if (!rows_apart || !dense_rows) dout = dout.contiguous();
       dw = at::empty({tokens, dim}, dout.options().dtype(dtype_of(sizes[2])));
@@ -255,9 +255,10 @@ PyObject *scaled_embedding(PyObject *, PyObject *const *args, Py_ssize_t n) {
         PyThreadState *state = PyEval_SaveThread();
         ~Released() { PyEval_RestoreThread(state); }
       } released;
+      weight = weight.resolve_neg();              // (a view with the sign pending, as of a conjugate's imag)
       if (!weight.is_contiguous() && (weight.stride(1) != 1 || weight.stride(0) < weight.size(1)))
         weight = weight.contiguous();
-      ids = ids.contiguous();
+      ids = ids.resolve_neg().contiguous();
       out = at::GradMode::is_enabled() && weight.requires_grad()
                 ? ScaledEmbedding::apply(weight, ids, scale, padding, dtype_code(to))
                 : lookup(weight, ids, scale, padding, dtype_code(to));
@@ -303,7 +304,7 @@ PyObject *adamw_step(PyObject *, PyObject *const *args, Py_ssize_t n) {
         throw Mismatch("parameters and gradients are tensors");
       const at::Tensor &p = THPVariable_Unpack(po);
       if (p.numel() != sizes[i] || dtype_code(p.scalar_type()) != dtypes[i] || p.device() != device ||
-          !p.is_contiguous())
+          !p.is_contiguous() || p.is_neg())
         throw Mismatch("parameter " + std::to_string(i) +
                        " no longer has the size, type, device or layout that the optimizer was made for");
       moved |= (int64_t)p.const_data_ptr() != planned[i];
@@ -319,8 +320,8 @@ PyObject *adamw_step(PyObject *, PyObject *const *args, Py_ssize_t n) {
         throw Mismatch("gradient " + std::to_string(i) + " must be a dense tensor of the parameter's type (" +
                        c10::toString(p.scalar_type()) + "), shape and device, got " +
                        c10::toString(g.scalar_type()) + " on " + g.device().str());
-      if (!g.is_contiguous()) {
-        g = g.detach().contiguous();
+      if (!g.is_contiguous() || g.is_neg()) {
+        g = g.detach().resolve_neg().contiguous();
         kept.push_back(g);
       }
       grad_at[i] = g.const_data_ptr();

@@ -65,8 +65,8 @@ class AdamW(object):
                 raise ValueError(f'parameter {i} is on {p.device}, the first one on {self.device}')
             if p.dtype not in _DTYPES:
                 raise TypeError(f'parameter {i} must be float32, bfloat16 or float16, got {p.dtype}')
-            if not p.is_contiguous():
-                raise ValueError(f'parameter {i} must be contiguous')
+            if not p.is_contiguous() or p.is_neg():
+                raise ValueError(f'parameter {i} must be contiguous (and no negated view)')
         self.state_bits, self.seed = state_bits, int(seed)
         self.betas, self.eps, self.lr = (float(betas[0]), float(betas[1])), float(eps), float(lr)
         self.weight_decay = decay
