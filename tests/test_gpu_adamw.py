@@ -274,6 +274,35 @@ def test_extreme_gradients(device, bits):
     assert ((moved + 3e-2).abs() < 3e-2 * 0.15).all()       # 8 bits: m and r are within 1/8 of theirs
 
 
+@pytest.mark.parametrize('dtype,size', [(torch.float32, 1e38), (torch.float32, 3e38), (torch.bfloat16, 2e38)])
+def test_the_largest_gradients(device, dtype, size):
+    """A first step moves every parameter by lr, whatever the gradient is: 8 u of it (1 / v_rcp), m, r and the
+    constants 4 u more, less than 16 u."""
+    from tracevae_amd.optim import AdamW
+    p = torch.zeros(600, dtype=dtype, device=device)
+    g = torch.full((600,), size, device=device).to(dtype)
+    g[::2] *= -1
+    g[100:300] *= 1e-3
+    opt = AdamW([p], weight_decay=0.0, state_bits=8, **HYPER)
+    opt.step([g])
+    w = opt.state['master'][:600] if 'master' in opt.state else p
+    want = -1e-2 * torch.sign(g).double()
+    assert ((w.double() - want).abs() <= 16 * U * 1e-2).all()
+
+
+def test_the_smallest_gradients_without_eps(device):
+    """m = 1e-39 and r = 3.2e-40 lie among fp32's numbers with steps of 2^-149: half a step is 2^-150 / 3.2e-40,
+    2.3e-6, of r, and 7e-7 of m, 7e-8 of their quotient's divisor."""
+    from tracevae_amd.optim import AdamW
+    p = torch.zeros(600, device=device)
+    g = torch.full((600,), 1e-38, device=device)
+    g[::2] *= -1
+    g[100:300] = 1e-3
+    opt = AdamW([p], lr=1e-2, weight_decay=0.0, eps=0.0, state_bits=8)
+    opt.step([g])
+    assert ((p.double() + 1e-2 * torch.sign(g).double()).abs() <= 1e-2 * 4e-6).all()
+
+
 def test_codes_of_tiny_and_mixed_magnitudes(device):
     """Blocks from 1e-36 to 1e15 in size, each with elements over 12 decades, zeros among them, and blocks
     of nothing but zeros: codes and scales equal to the definition's."""
