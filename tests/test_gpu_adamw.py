@@ -405,6 +405,25 @@ def test_state_dict_continues_bit_for_bit(device):
             assert torch.equal(opt.state[k].view(torch.uint8), again.state[k].view(torch.uint8))
 
 
+def test_a_captured_learning_rate(device):
+    """A rate whose store was captured is set by every replay; set_lr to the rate before is a store again."""
+    from tracevae_amd.optim import AdamW
+    params = _params([(600,)], torch.float32, device, 63)
+    opt = AdamW(params, weight_decay=0.01, **HYPER)
+    twin = Twin(opt, [0.01])
+    twin.step(_grads(params, 64))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.set_lr(1e-3)
+    for lr in (1e-2, 1e-3):
+        opt.set_lr(lr)
+        twin.step(_grads(params, 65))
+        graph.replay()
+        opt.set_lr(lr)
+        twin.step(_grads(params, 66))
+
+
 @pytest.mark.parametrize('bits', [32, 8])
 @pytest.mark.parametrize('how', ['deepcopy', 'save'])
 def test_a_copy_of_an_optimizer_stands_alone(device, bits, how):

@@ -69,6 +69,7 @@ class AdamW(object):
                 raise ValueError(f'parameter {i} must be contiguous (and no negated view)')
         self.state_bits, self.seed = state_bits, int(seed)
         self.betas, self.eps, self.lr = (float(betas[0]), float(betas[1])), float(eps), float(lr)
+        self._captured_lr = False
         self.weight_decay = decay
         self._make_arrays()
         lib = hip.lib()
@@ -160,11 +161,14 @@ class AdamW(object):
 
     # -- hyper-parameters and state ----------------------------------------------------
     def set_lr(self, lr: float) -> None:
-        """The learning rate of the steps queued behind this call (a store on the current stream)."""
+        """The learning rate of the steps queued behind this call (a store on the current stream; captured, a
+        store of every replay)."""
         lr = float(lr)
         if not 0.0 <= lr < float('inf'):
             raise ValueError(f'the learning rate must be finite and not negative, got {lr}')
-        if lr != self.lr:
+        # (behind a captured store, replays change the device's rate without the host)
+        self._captured_lr |= torch.cuda.is_current_stream_capturing()
+        if lr != self.lr or self._captured_lr:
             self.lr = lr
             self._lr.fill_(lr)
 
