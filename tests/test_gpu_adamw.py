@@ -405,6 +405,30 @@ def test_state_dict_continues_bit_for_bit(device):
             assert torch.equal(opt.state[k].view(torch.uint8), again.state[k].view(torch.uint8))
 
 
+def test_a_state_of_another_seed_is_refused(device):
+    from tracevae_amd.optim import AdamW
+
+    def make(seed, bits=8):
+        return AdamW([torch.ones(300, device=device)], state_bits=bits, seed=seed, **HYPER)
+
+    a = make(2 ** 40 + 5)
+    a.step([torch.randn(300, device=device)])
+    state = a.state_dict()
+    for seed in (5, 2 ** 32 + 5):                         # (the low 32 bits are the seed)
+        b = make(seed)
+        b.load_state_dict(state)
+        assert b.steps == 1
+    b = make(6)
+    before = b.state_dict()
+    with pytest.raises(ValueError, match='seed'):
+        b.load_state_dict(state)
+    for k, v in b.state_dict().items():
+        assert v == 0 if k == 'step' else torch.equal(v.view(torch.uint8), before[k].view(torch.uint8))
+    del state['seed']                                     # one that names none is taken
+    b.load_state_dict(state)
+    assert b.steps == 1 and set(make(1, 32).state_dict()) == {'exp_avg', 'exp_avg_sq', 'step'}
+
+
 def test_a_captured_learning_rate(device):
     """A rate whose store was captured is set by every replay; set_lr to the rate before is a store again."""
     from tracevae_amd.optim import AdamW

@@ -183,12 +183,21 @@ class AdamW(object):
         return dict(self._state)
 
     def state_dict(self) -> Dict[str, object]:
-        return dict({k: v.clone() for k, v in self._state.items()}, step=self.steps)
+        """Copies of the buffers, the step and, of 8-bit moments, the low 32 bits of the seed."""
+        out = dict({k: v.clone() for k, v in self._state.items()}, step=self.steps)
+        if self.state_bits == 8:
+            out['seed'] = torch.tensor([self.seed & 0xffffffff])
+        return out
 
     def load_state_dict(self, state: Dict[str, object]) -> None:
-        """Copies the buffers of a `state_dict()` of the same parameters and `state_bits`."""
+        """Copies the buffers of a `state_dict()` of the same parameters, `state_bits` and, if the state names one,
+        `seed` (with another one the codes of the steps to come would be others)."""
+        state = dict(state)
+        seed = state.pop('seed', None) if self.state_bits == 8 else None
         if set(state) != set(self._state) | {'step'}:
             raise ValueError(f'the state has {sorted(state)}, expected {sorted(self._state)} and step')
+        if seed is not None and int(seed) & 0xffffffff != self.seed & 0xffffffff:
+            raise ValueError(f'the state is that of seed {int(seed)}, this optimizer has {self.seed}')
         for k, v in self._state.items():
             if tuple(state[k].shape) != tuple(v.shape) or state[k].dtype != v.dtype:
                 raise ValueError(f'{k} must be {v.dtype} of {tuple(v.shape)}, got {state[k].dtype} '
