@@ -167,6 +167,36 @@ def test_steps_with_and_without_clipping_in_turn(device, bits):
 
 
 @pytest.mark.parametrize('bits', [32, 8])
+@pytest.mark.parametrize('chunks', [64, 65, 127, 128, 129])
+def test_around_the_one_launch_limit(device, bits, chunks):
+    """Up to 128 chunks an unclipped step is one launch whose last workgroup counts it: against the formula, and
+    captured and replayed against eager steps."""
+    from tracevae_amd.optim import AdamW
+    shapes = [(4096 * (chunks - 3) - 5,), (100,), (4097,)]
+    params = _params(shapes, torch.float32, device, 71)
+    opt = AdamW(params, weight_decay=0.01, state_bits=bits, **HYPER)
+    twin = Twin(opt, [0.01] * 3)
+    for k in range(3):
+        twin.step(_grads(params, 72 + k))
+    copies = [p.clone() for p in params]
+    other = AdamW(copies, weight_decay=0.01, state_bits=bits, **HYPER)
+    other.load_state_dict(opt.state_dict())
+    g = _grads(params, 75)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step(g)
+    for k in range(3):
+        for x, y in zip(g, _grads(params, 76 + k)):
+            x.copy_(y)
+        graph.replay()
+        other.step(g)
+        assert opt.steps == other.steps == 4 + k
+        for a, b in zip([*params, *opt.state.values()], [*copies, *other.state.values()]):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.parametrize('bits', [32, 8])
 def test_eps_of_zero_leaves_the_padding_zero(device, bits):
     from tracevae_amd.optim import AdamW
     params = _params([(255,), (3, 5), (1,), (4097,)], torch.bfloat16, device, 31)

@@ -123,6 +123,32 @@ def test_no_rows_and_nothing_but_padding(device):
         _check(w, torch.full((500,), 3), 2.0, 3, out_dtype, torch.randn(500, 24).to(out_dtype), device)
 
 
+@pytest.mark.parametrize('rows,vocab,dim', [(0, 70, 24), (5, 300, 3), (128, 300, 72), (129, 300, 72),
+                                           (700, 1501, 513), (300, 70001, 130), (2049, 300000, 33),
+                                           (70000, 200001, 24), (20000, 5, 8)])
+@pytest.mark.parametrize('kind', ['zipf', 'same', 'padding'])
+def test_every_row_of_the_table_gradient_is_written(device, rows, vocab, dim, kind):
+    """Into memory full of NaN, with a row before and a row behind that stay as they are, and so does what lies
+    behind the workspace."""
+    from tracevae_amd import hip
+    codes = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+    g = torch.Generator().manual_seed(rows + vocab)
+    ids = _ids(kind, rows, vocab, g)
+    for table, rt in TYPES[:4]:
+        d = torch.randn(rows, dim, generator=g).to(rt)
+        need = hip.query('tv_scaled_embedding_bwd_workspace_bytes', rows, dim, vocab)
+        ws = torch.full((need + 256,), 255, dtype=torch.uint8, device=device)
+        around = torch.full((vocab + 2, dim), math.nan, dtype=table, device=device)
+        ids_d, d_d = ids.to(device), d.to(device)
+        hip.call('tv_scaled_embedding_bwd', rows, dim, vocab, codes[table], codes[rt], hip.ptr(ids_d), -1, 0.5,
+                 hip.ptr(d_d), dim, around[1:].data_ptr(), hip.ptr(ws), need)
+        _, dw, size, count = _reference(torch.zeros(vocab, dim), ids, 0.5, None, d)
+        got = around.cpu().double()
+        assert torch.isnan(got[0]).all() and torch.isnan(got[-1]).all() and (ws[need:] == 255).all()
+        assert ((got[1:-1] - dw).abs() <= (count + 1) * U * size + _half_step(table) * dw.abs() * (1 + 1e-3)
+                + (2.0 ** -25 if torch.float16 in (table, rt) else 0.0)).all()
+
+
 def test_infinities_and_nan_stay_in_their_rows(device):
     """inf / NaN in rows of the table that no token names, and in the gradient of padded rows."""
     from tracevae_amd import ops
