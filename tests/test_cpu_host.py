@@ -407,3 +407,22 @@ def test_nan_restart_loop(tmp_path):
     with pytest.raises(NANLossError):
         run_with_nan_restart(job_factory(99, 1), str(out), log=messages.append)
     assert len(calls) == 11                                    # the first try + 10 restarts
+
+
+def test_the_library_is_built_where_there_is_no_torch():
+    """`make` plans the library alone where PYTHON has no torch, both where it has; the extension module asked for
+    by name is refused there."""
+    import subprocess
+
+    def plan(*args):
+        return subprocess.run(['make', '-n', '-B', '-C', os.path.join(ROOT, 'tracevae_amd', 'csrc'), *args],
+                              capture_output=True, text=True)
+
+    without, with_torch = plan('PYTHON=/bin/false'), plan(f'PYTHON={sys.executable}')
+    assert without.returncode == 0 and with_torch.returncode == 0
+    assert 'libtracevae_hip.so' in without.stdout and 'torch_host.cpp' not in without.stdout
+    assert 'libtracevae_hip.so' in with_torch.stdout and 'torch_host.cpp' in with_torch.stdout
+    csrc = os.path.join(ROOT, 'tracevae_amd', 'csrc')
+    asked = subprocess.run(['make', '-C', csrc, '-W', 'torch_host.cpp', '_torch_host.so', 'PYTHON=/bin/false'],
+                           capture_output=True, text=True)
+    assert asked.returncode != 0 and 'needs torch' in asked.stdout
