@@ -167,7 +167,8 @@ class AdamW(object):
         if not 0.0 <= lr < float('inf'):
             raise ValueError(f'the learning rate must be finite and not negative, got {lr}')
         # (behind a captured store, replays change the device's rate without the host)
-        self._captured_lr |= torch.cuda.is_current_stream_capturing()
+        with torch.cuda.device(self.device):
+            self._captured_lr |= torch.cuda.is_current_stream_capturing()
         if lr != self.lr or self._captured_lr:
             self.lr = lr
             self._lr.fill_(lr)
