@@ -496,14 +496,16 @@ int tv_embedding_bwd(int64_t rows, int64_t dim, int64_t num_operations, const in
 
 /* Rows of a table by token id, times a scale, and the gradient of the table by sorted tokens (the
  * operation embedding, model/operation_embedding.py:21-25, as tables of many tokens need it):
- *   out[r]     = round(scale * weight[ids[r]])   rows of zeros for ids outside [0, num_tokens) and
- *                                                for padding_id (-1: none)
+ *   out[r]     = round(fp32(scale * weight[ids[r]]))   rows of zeros for ids outside [0, num_tokens)
+ *                                                      and for padding_id (-1: none)
  *   dweight[v] = round(scale * sum over r with ids[r] = v of dout[r]); every row is written
  * weight / out types (TV_DTYPE_*): equal, or an fp32 table with 16-bit rows; dout has out's type,
  * dweight weight's, [num_tokens, dim] dense.  Row strides in elements; no alignment beyond the
  * type's is needed (rows at multiples of 16 bytes are the fastest).  Sums are fp32 in a fixed
- * order, rounded once.  num_tokens <= 2^29, dim <= 65536, and rows * L < 2^33, where L is dim / 4
- * rounded up to 16, 32 or a multiple of 64 (2^29 rows of up to 64 columns, 2^25 of 1024).
+ * order, and so is their product with the fp32 scale, which is then rounded to the type (in fp16 rows
+ * of less than 8 columns it may be rounded once).  num_tokens <= 2^29, dim <= 65536, and
+ * rows * L < 2^33, where L is dim / 4 rounded up to 16, 32 or a multiple of 64 (2^29 rows of up to 64
+ * columns, 2^25 of 1024).
  * Workspace of the backward pass: 16-byte aligned, tv_scaled_embedding_bwd_workspace_bytes (0 for up
  * to 128 rows). */
 int tv_scaled_embedding_fwd(int64_t rows, int64_t dim, int64_t num_tokens, int weight_dtype,
@@ -738,7 +740,8 @@ int tv_optim_step_guarded(int kind, int64_t n, float *param, const float *grad, 
  *     of (seed, step, element): same seed, same bits.  A sqrt(v) that is positive in fp32 keeps a
  *     positive code; an infinite or NaN moment becomes the NaN code and leaves its neighbours alone;
  *     a block whose scale would be below 2^-100 is stored as zeros.  Everything up to codes and scales
- *     is float64, m as two products and a sum, each rounded.
+ *     is float64, m as two products and a sum, each rounded, and sqrt(v) to 2^-47 of itself: scale2 of
+ *     one block in some 10 million is the neighbouring fp32 number.
  *   master: fp32, needed if any parameter has 16 bits (otherwise NULL).
  *
  * tv_adamw_plan writes the table of tensors and chunks into HOST memory; the caller keeps it and a

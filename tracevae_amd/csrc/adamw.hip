@@ -10,8 +10,8 @@
 // from step to step, travel as kernel arguments.  Everything is elementwise and bound by HBM: 28 bytes
 // per fp32 parameter with 32-bit moments, 16.06 with 8-bit ones, 30 / 18.06 per 16-bit one with its
 // master, and the gradient once more for the norm.  Measured (kernels alone): 343 million bf16
-// parameters, 32 bits: 1.59 ms, 10.3 GB at 6.5 TB/s, norm 0.11 ms; fp32, 8 bits: 0.93 ms, 5.5 GB at 5.9
-// TB/s; 14 million in 152 tensors: 60 us + 14 + 5 for the norm, 8 bits 41 + 14 + 4; 62 000 in 16
+// parameters, 32 bits: 1.59 ms, 10.3 GB at 6.5 TB/s, norm 0.11 ms; fp32, 8 bits: 0.93-0.95 ms, 5.5 GB at 5.9
+// TB/s; 14 million in 152 tensors: 60 us + 14 + 5 for the norm, 8 bits 42 + 14 + 4; 62 000 in 16
 // tensors: 4.3 us.
 //
 // 8-bit moments: m / s_m and sqrt(v) / s_r in e4m3 with s = max over the block / 448, so that the

@@ -1221,13 +1221,13 @@ def embedding(weight, ids, extra_cols: int = 0):
 
 def scaled_embedding(weight, ids, scale: float = 1.0, padding_idx: Optional[int] = None,
                      out_dtype: Optional[torch.dtype] = None):
-    """`scale * weight[ids]`, rounded once to `out_dtype` (default: the table's type; a 16-bit type
-    for an fp32 table), of shape `ids.shape + (dim,)`.  Ids outside the table and ids equal to
+    """`scale * weight[ids]`, computed in fp32 and rounded to `out_dtype` (default: the table's type; a
+    16-bit type for an fp32 table), of shape `ids.shape + (dim,)`.  Ids outside the table and ids equal to
     `padding_idx` (which is not counted from the end) give rows of zeros and no gradient.  The
     gradient of the table is summed in fp32 over its tokens in the order of `ids`, whatever their
     number (`tv_scaled_embedding_bwd`), and is dense; once differentiable, and in reverse mode only (a
-    tangent of the table or of the rows' gradient is refused).  A captured backward pass that leads to a tensor
-    which a living eager graph holds is refused (autograd would end the process).
+    tangent of the table or of the rows' gradient is refused).  A captured backward pass that leads to
+    a tensor which a living eager graph holds is refused (autograd would end the process).
     `weight`: [tokens, dim] in fp32, bf16 or fp16 with contiguous, possibly strided rows."""
     return hip.host().scaled_embedding(weight, ids, scale, padding_idx, out_dtype)
 
