@@ -244,6 +244,19 @@ def test_gradients_with_the_sign_pending(device, bits):
 
 
 @pytest.mark.parametrize('bits', [32, 8])
+def test_zero_gradients_without_memory(device, bits):
+    """autograd's zeros, whose address is null, are a gradient of zeros and not the absence of one."""
+    from tracevae_amd.optim import AdamW
+    params = _params([(300,), (17, 3)], torch.bfloat16, device, 67)
+    opt = AdamW(params, weight_decay=0.01, state_bits=bits, **HYPER)
+    twin = Twin(opt, [0.01] * 2)
+    twin.step(_grads(params, 68))
+    for k, clip in enumerate((None, 1.0)):
+        g = [torch.zeros_like(params[0]), _grads(params, 69 + k)[1]]
+        twin.step(g, clip, [torch._efficientzerotensor((300,), dtype=torch.bfloat16, device=device), g[1]])
+
+
+@pytest.mark.parametrize('bits', [32, 8])
 def test_more_tensors_than_one_launch_takes(device, bits):
     from tracevae_amd.optim import AdamW
     shapes = [(1 + (i * 37) % 300,) for i in range(900)] + [(5000,)]

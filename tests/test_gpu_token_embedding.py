@@ -299,6 +299,19 @@ def test_views_with_the_opposite_sign(device, dim):
         assert torch.equal(dw, want)
 
 
+def test_zeros_without_memory(device):
+    from tracevae_amd import ops
+    x = torch.randn(30, 6, device=device, requires_grad=True)
+    ids = torch.arange(600, device=device) % 30
+    for rows in (60, 600):
+        zeros = torch._efficientzerotensor((rows, 6), device=device)
+        assert zeros.data_ptr() == 0
+        (dw,) = torch.autograd.grad(ops.scaled_embedding(x, ids[:rows], 2.0), x, zeros)
+        assert torch.equal(dw, torch.zeros_like(x))
+    out = ops.scaled_embedding(torch._efficientzerotensor((30, 6), device=device), ids, 2.0)
+    assert torch.equal(out, torch.zeros(600, 6, device=device))
+
+
 def test_more_than_2_to_the_31_elements(device):
     """bf16 rows of 2^21 + 5 tokens by 1030 columns: positions beyond 32 bits in the rows and in their
     gradient (4.3 GB each)."""

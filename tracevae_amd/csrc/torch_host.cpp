@@ -107,6 +107,12 @@ void refuse_tangent(const at::Tensor &t, const char *what) {
                               " carries a tangent, forward mode is not implemented");
 }
 
+// What a view or a tensor without memory stands for, in memory: a sign that is pending (the imaginary part of a
+// conjugate), autograd's zeros, whose address is null.
+at::Tensor in_memory(const at::Tensor &t) {
+  return t._is_zerotensor() ? t.clone() : t.resolve_neg();
+}
+
 // (behind the checks of scaled_embedding below: a [tokens, dim] table with contiguous rows, contiguous
 // int64 ids on its device, types that go together)
 at::Tensor lookup(const at::Tensor &weight, const at::Tensor &ids, double scale, int64_t padding_id, int64_t out_code) {
@@ -154,7 +160,7 @@ class ScaledEmbedding : public torch::autograd::Function<ScaledEmbedding> {
     at::Tensor dw;
     {
       const at::AutoGradMode no_grad(false);
-      at::Tensor dout = grads[0].resolve_neg().reshape({rows, dim});
+      at::Tensor dout = in_memory(grads[0]).reshape({rows, dim});
       const bool rows_apart = rows <= 1 || dout.stride(0) >= dim, dense_rows = dim <= 1 || dout.stride(1) == 1;
       if (!rows_apart || !dense_rows) dout = dout.contiguous();
       dw = at::empty({tokens, dim}, dout.options().dtype(dtype_of(sizes[2])));
@@ -255,10 +261,10 @@ PyObject *scaled_embedding(PyObject *, PyObject *const *args, Py_ssize_t n) {
         PyThreadState *state = PyEval_SaveThread();
         ~Released() { PyEval_RestoreThread(state); }
       } released;
-      weight = weight.resolve_neg();              // (a view with the sign pending, as of a conjugate's imag)
+      weight = in_memory(weight);
       if (!weight.is_contiguous() && (weight.stride(1) != 1 || weight.stride(0) < weight.size(1)))
         weight = weight.contiguous();
-      ids = ids.resolve_neg().contiguous();
+      ids = in_memory(ids).contiguous();
       out = at::GradMode::is_enabled() && weight.requires_grad()
                 ? ScaledEmbedding::apply(weight, ids, scale, padding, dtype_code(to))
                 : lookup(weight, ids, scale, padding, dtype_code(to));
@@ -320,8 +326,8 @@ PyObject *adamw_step(PyObject *, PyObject *const *args, Py_ssize_t n) {
         throw Mismatch("gradient " + std::to_string(i) + " must be a dense tensor of the parameter's type (" +
                        c10::toString(p.scalar_type()) + "), shape and device, got " +
                        c10::toString(g.scalar_type()) + " on " + g.device().str());
-      if (!g.is_contiguous() || g.is_neg()) {
-        g = g.detach().resolve_neg().contiguous();
+      if (!g.is_contiguous() || g.is_neg() || g._is_zerotensor()) {
+        g = in_memory(g.detach()).contiguous();
         kept.push_back(g);
       }
       grad_at[i] = g.const_data_ptr();
