@@ -591,6 +591,20 @@ def test_the_plan_of_a_captured_step_outlives_a_move(device, bits):
     assert torch.isfinite(first).all() and len(opt._captured_plans) == 1
 
 
+def test_a_changed_list_of_parameters_is_refused(device):
+    from tracevae_amd.optim import AdamW
+    params = _params([(600,), (5,)], torch.float32, device, 83)
+    opt = AdamW(params, **HYPER)
+    for change in (lambda: opt.params.append(params[0]), lambda: opt.params.clear()):
+        keep = list(opt.params)
+        change()
+        with pytest.raises(ValueError, match='made for 2'):
+            opt.step([None] * len(opt.params))
+        opt.params[:] = keep
+    opt.step(_grads(params, 84))
+    assert opt.steps == 1
+
+
 def test_on_a_stream_of_its_own(device):
     from tracevae_amd.optim import AdamW
     params = _params([(100000,)], torch.float32, device, 26)

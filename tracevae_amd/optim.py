@@ -230,6 +230,8 @@ class AdamW(object):
         if guard_host is not None and (guard_host.dtype != torch.float32 or guard_host.numel() != 1
                                        or guard_host.is_cuda):
             raise TypeError('guard_host must be one float32 in pinned host memory')
+        if len(self.params) != len(self.offsets):
+            raise ValueError(f'{len(self.params)} parameters, but the optimizer was made for {len(self.offsets)}')
         clip = float(global_clip_norm or 0.0)
         if grads is not None and type(grads) is not list:
             grads = list(grads)
