@@ -59,8 +59,7 @@ void *stream_of(const at::Tensor &t) {
   return (void *)c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream();
 }
 
-bool capturing(const c10::Stream &s) {
-  const hipStream_t stream = c10::hip::HIPStreamMasqueradingAsCUDA(s).stream();
+bool capturing(hipStream_t stream) {
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
   if (stream == nullptr) return false;            // (the default stream cannot be captured)
   if (hipStreamIsCapturing(stream, &status) != hipSuccess) {
@@ -69,6 +68,7 @@ bool capturing(const c10::Stream &s) {
   }
   return status == hipStreamCaptureStatusActive;
 }
+bool capturing(const c10::Stream &s) { return capturing(c10::hip::HIPStreamMasqueradingAsCUDA(s).stream()); }
 
 // Autograd runs a node on the stream on which it was made and lets that stream wait for the node before it.
 // In a captured backward pass a node from outside the capture - the accumulator of a leaf that an eager
@@ -110,7 +110,7 @@ void refuse_tangent(const at::Tensor &t, const char *what) {
 // What a view or a tensor without memory stands for, in memory: a sign that is pending (the imaginary part of a
 // conjugate), autograd's zeros, whose address is null.
 at::Tensor in_memory(const at::Tensor &t) {
-  return t._is_zerotensor() ? t.clone() : t.resolve_neg();
+  return t._is_zerotensor() ? t.clone() : t.is_neg() ? t.resolve_neg() : t;
 }
 
 // (behind the checks of scaled_embedding below: a [tokens, dim] table with contiguous rows, contiguous
@@ -277,7 +277,8 @@ PyObject *scaled_embedding(PyObject *, PyObject *const *args, Py_ssize_t n) {
 // moment1, moment2, scale1, scale2, master, control, clip, norm, seed, guard, guard_kind, guard_host,
 // workspace, workspace_bytes, stream, device): tv_adamw_step with the gradients' addresses.  dtypes (int), sizes
 // and planned (int64: the parameters' addresses in the plan) are arrays of the optimizer, addresses is
-// its int64 scratch.  False: a parameter is not where the plan has it, nothing was done.
+// its int64 scratch.  False: a parameter is not where the plan has it, nothing was done.  None: the step was
+// captured, with the plan's address.
 PyObject *adamw_step(PyObject *, PyObject *const *args, Py_ssize_t n) {
   if (n != 25 || !PyList_Check(args[0]) || !(args[1] == Py_None || PyList_Check(args[1]))) {
     PyErr_SetString(PyExc_TypeError, "adamw_step takes a list of parameters, a list of gradients or None, and 23 more");
@@ -297,6 +298,11 @@ PyObject *adamw_step(PyObject *, PyObject *const *args, Py_ssize_t n) {
   PyObject *params = args[0], *grads = args[1] == Py_None ? nullptr : args[1];
   const Py_ssize_t count = PyList_GET_SIZE(params);
   const at::Device device(at::kCUDA, (at::DeviceIndex)(intptr_t)a[24]);
+  const int64_t planned_count = ((const int64_t *)a[6])[1];        // (head of the plan: magic, count)
+  if (count != planned_count) {
+    PyErr_Format(PyExc_ValueError, "%zd parameters, but the optimizer was made for %lld", count, (long long)planned_count);
+    return nullptr;
+  }
   if (grads && PyList_GET_SIZE(grads) != count) {
     PyErr_Format(PyExc_ValueError, "%zd gradients for %zd parameters", PyList_GET_SIZE(grads), count);
     return nullptr;
@@ -342,6 +348,7 @@ PyObject *adamw_step(PyObject *, PyObject *const *args, Py_ssize_t n) {
       const at::Tensor &p = THPVariable_Unpack(PyList_GET_ITEM(params, i));
       if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
     }
+    if (capturing((hipStream_t)a[23])) Py_RETURN_NONE;
     Py_RETURN_TRUE;
   });
 }

@@ -230,23 +230,26 @@ class AdamW(object):
         if guard_host is not None and (guard_host.dtype != torch.float32 or guard_host.numel() != 1
                                        or guard_host.is_cuda):
             raise TypeError('guard_host must be one float32 in pinned host memory')
-        if len(self.params) != len(self.offsets):
-            raise ValueError(f'{len(self.params)} parameters, but the optimizer was made for {len(self.offsets)}')
         clip = float(global_clip_norm or 0.0)
         if grads is not None and type(grads) is not list:
             grads = list(grads)
-        capturing = torch.cuda.is_current_stream_capturing()
-        if capturing and not any(p is self._plan for p in self._captured_plans):
-            self._captured_plans.append(self._plan)
         step = hip.host().adamw_step
-        while not step(self.params, grads, *self._fixed, clip,
-                       self.grad_norm.data_ptr() if clip else None, self.seed, hip.ptr(guard),
-                       guard_kind if guard is not None else 0,
-                       guard_host.data_ptr() if guard_host is not None else None,
-                       self._workspace.data_ptr(), self._workspace.numel() * 8, hip.stream(),
-                       self.device.index):
+        while True:
+            done = step(self.params, grads, *self._fixed, clip,
+                        self.grad_norm.data_ptr() if clip else None, self.seed, hip.ptr(guard),
+                        guard_kind if guard is not None else 0,
+                        guard_host.data_ptr() if guard_host is not None else None,
+                        self._workspace.data_ptr(), self._workspace.numel() * 8, hip.stream(),
+                        self.device.index)
+            if done:
+                break
+            if done is None:
+                # captured: the plan is read by every replay
+                if not any(p is self._plan for p in self._captured_plans):
+                    self._captured_plans.append(self._plan)
+                break
             # a parameter is not where it was
-            if capturing:
+            if torch.cuda.is_current_stream_capturing():
                 raise hip.HipLibraryError('a parameter has moved since the last step: take one '
                                           'eager step before capturing')
             self._make_plan()
